@@ -47,6 +47,13 @@ class LlamaBlockStruct(C.Structure):
                 ("w_o", C.c_void_p), ("w_gate_up", C.c_void_p), ("w_down", C.c_void_p), ("rope_base", C.c_float)]
 
 
+class PagedCacheStruct(C.Structure):
+    """catena_paged_cache_t (include/catena_b200.h)."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p), ("n_pages", C.c_uint64),
+                ("page_size", C.c_uint64), ("n_seqs", C.c_uint64), ("max_pages", C.c_uint64), ("n_kv_heads", C.c_uint64),
+                ("head_dim", C.c_uint64)]
+
+
 class CatenaError(RuntimeError):
     def __init__(self, status, what=""):
         self.status = int(status)
@@ -162,6 +169,17 @@ def lib():
     proto("catena_b200_add_bf16_into", st, [vp, vp, vp, u64])
     proto("catena_b200_linear_swiglu_bf16_into", st, [vp, vp, vp, vp, u64, u64, u64])
     proto("catena_b200_linear_bf16_into", st, [vp, vp, vp, vp, u64, u64, u64])
+    pcache = C.POINTER(PagedCacheStruct)
+    proto("catena_b200_rope_angles_f32_into", st, [f32, u64, u64, u64, vp])
+    proto("catena_b200_rope_append_paged_bf16_into", st, [pcache, vp, u64, vp, u64, vp, vp, u64, u64, vp])
+    proto("catena_b200_attn_decode_paged_workspace_bytes", u64, [pcache, u64, C.c_int])
+    proto("catena_b200_attn_decode_paged_bf16_into", st, [pcache, vp, vp, u64, f32, vp, vp, vp, u64])
+    proto("catena_b200_kv_evict_paged_workspace_bytes", u64, [pcache, u64])
+    proto("catena_b200_kv_evict_paged_bf16_into", st, [pcache, vp, u64, u64, vp, u64, vp, vp, vp, vp, u64])
+    proto("catena_b200_beam_select_workspace_bytes", u64, [u64, u64, u64, u64])
+    for name in ["catena_b200_beam_select_f32_into", "catena_b200_beam_select_bf16_into"]:
+        proto(name, st, [vp, u64, vp, u64, u64, u64, u64, vp, vp, vp, vp, u64])
+    proto("catena_b200_beam_reorder_paged_bf16_into", st, [pcache, vp, u64, vp, vp, vp, vp, vp])
     proto("catena_b200_debug_set_cta_limit", None, [C.c_int])
     proto("catena_b200_sum_f32_noalloc", st, [vp, u64, vp])
     proto("catena_b200_debug_set_gemm_pair", None, [C.c_int])

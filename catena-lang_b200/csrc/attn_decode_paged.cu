@@ -1,0 +1,497 @@
+// Attention of one new token per sequence over a paged key/value cache, sequences of any lengths.
+//   s_j = scale * (q . k_j)     o = sum_j p_j v_j / sum_j p_j     p_j = exp(s_j - max s)
+// and, when asked for, weights_out[j] = weights_in[j] + sum over the group's query heads of p_j / sum p.
+// The exponential is the true one (ex2.approx in base 2), not math.exp-approx: that polynomial is not multiplicative, so it would
+// need the row's maximum before the first probability and with it a second pass over the scores.  Here one pass carries a running
+// maximum and sum.  q, k, v are bf16; scores, maxima, sums and outputs are f32 until the one rounding of o.  A probability enters
+// the second product as a bf16 pair (p rounded, and what the rounding left): with a single bf16 every p would be off by up to 2^-9
+// of itself, which for a row that looks at few keys is as much as the rounding of o.
+//
+// Bound: HBM.  A row costs 4 d bytes and 4 d flops per query head of the group, so even 16 heads (64 flops per 4 bytes) stay far
+// under the tensor rate; mma.sync on 16-row pieces feeds from a ring that each warp fills for itself with cp.async, and no warp
+// waits for another while it streams.
+//
+// Split: all (sequence, kv head) units' rows are cut into tiles of 64 (d = 128) or 128 (d = 64) keys, and CTA c of C takes tiles
+// [c T / C, (c + 1) T / C) of the T there are (C = T when there are fewer tiles than CTAs): every CTA gets the same number of tiles whatever the lengths are, and the lengths
+// need not be known on the host.  A unit that lies inside one CTA is finished there; of a unit cut by CTA boundaries every CTA
+// leaves (max, sum, unnormalised output), joined in ascending order by the second launch.  The order of every sum depends on
+// the lengths and the number of SMs only: equal calls give equal bits.
+#include "catena_math.cuh"
+#include "paged.cuh"
+
+namespace catena {
+namespace paged {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStages = 3;                      // tiles in flight per warp
+constexpr int kCtasPerSm = 2;
+constexpr uint32_t kStageBytes = 8192;          // a warp's keys and values of one tile
+constexpr float kLazy = 8.0f;                   // probabilities may reach 2^8 before the running maximum is raised
+
+template <int D> struct Shape {
+    static constexpr int kKeys = D == 128 ? 16 : 32;          // keys per warp and tile
+    static constexpr int kTile = kKeys * kWarps;
+    static constexpr int kPitch = D + 4;                      // floats per head of the merge buffer: conflict-free for (8 d, 4 heads)
+    static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+    static constexpr uint32_t kMerge = kWarps * 8 * kPitch * 4;
+    static constexpr uint32_t kSmem = kRing + kMerge + kWarps * 8 * 2 * 4;
+};
+
+// What a CTA left behind: of the segment that began its unit and did not finish it (slot 1), of the one that continues a unit
+// begun by an earlier CTA (slot 0).  first.x: 1 = slot 1 holds the beginning of a unit; y: unit; z: tiles of the unit in later CTAs
+struct Partials {
+    uint4* first;       // [C]
+    float2* ml;         // [C][2][16]   (max in base 2, sum)
+    float* o;           // [C][2][hq / hkv][D]
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
+}
+
+// tiles of one head of all sequences; whole CTA
+template <int TILE>
+__device__ __forceinline__ uint64_t count_tiles(const View& c, uint64_t* sums) {
+    uint64_t mine = 0;
+    for (uint32_t b = threadIdx.x; b < c.n_seqs; b += kThreads) mine += (c.length(b) + TILE - 1) / TILE;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, off);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    uint64_t all = 0;
+    for (int w = 0; w < kWarps; ++w) all += sums[w];
+    __syncthreads();
+    return all;
+}
+
+// a position in the list of all tiles: unit (b, h), tile of the unit, rows of the sequence
+template <int TILE>
+struct Cursor {
+    uint32_t b, h, tile, n;
+    __device__ __forceinline__ uint32_t tiles() const { return (n + TILE - 1) / TILE; }
+    __device__ __forceinline__ void next(const View& c) {
+        if (++tile < tiles()) return;
+        tile = 0;
+        if (++h < c.hkv) return;
+        h = 0;
+        do {
+            ++b;
+            n = b < c.n_seqs ? c.length(b) : 1u;
+        } while (n == 0);
+    }
+};
+
+template <int D, int NT, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel(View c, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ o,
+                                                                                 uint32_t hq, float scale_log2, Partials part,
+                                                                                 float* __restrict__ scores, float2* __restrict__ stats) {
+    using S = Shape<D>;
+    constexpr int KEYS = S::kKeys, TILE = S::kTile, SUB = KEYS / 16, CH = D / 8;     // CH: 16-byte pieces of a row
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* merge = reinterpret_cast<float*>(smem + S::kRing);
+    float2* merge_ml = reinterpret_cast<float2*>(smem + S::kRing + S::kMerge);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const uint32_t group = hq / c.hkv, C = gridDim.x, cta = blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
+
+    for (uint32_t b = cta; b < c.n_seqs; b += C) {                 // a sequence without rows: zeros
+        if (c.length(b) != 0) continue;
+        for (uint32_t i = tid; i < hq * D / 8; i += kThreads) reinterpret_cast<uint4*>(o + (size_t)b * hq * D)[i] = make_uint4(0, 0, 0, 0);
+    }
+    const uint64_t total = count_tiles<TILE>(c, reinterpret_cast<uint64_t*>(merge)) * c.hkv;
+    const uint64_t n_cta = total < C ? total : C;                  // CTAs with work: each has a tile at least
+    const uint64_t t0 = cta < n_cta ? cta * total / n_cta : 0, t1 = cta < n_cta ? (cta + 1) * total / n_cta : 0;
+    if (t0 == t1) {
+        if (tid == 0) part.first[cta] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    Cursor<TILE> load;                                             // the tile that is loaded next
+    {
+        // the sequence that holds tile t0: warps look at 32 sequences at a time
+        uint64_t before = 0;
+        uint32_t b0 = 0, found = 0;
+        for (; b0 < c.n_seqs; b0 += 32) {
+            const uint32_t b = b0 + lane;
+            uint32_t mine = b < c.n_seqs ? (c.length(b) + TILE - 1) / TILE : 0u, x = mine;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, off);
+                if (lane >= (uint32_t)off) x += y;
+            }
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, (before + x) * c.hkv > t0);
+            if (hit) {
+                found = __ffs(hit) - 1;
+                before += __shfl_sync(0xFFFFFFFFu, x - mine, found);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, x, 31);
+        }
+        load.b = b0 + found;
+        load.n = c.length(load.b);
+        const uint32_t rest = (uint32_t)(t0 - before * c.hkv);
+        load.h = rest / load.tiles();
+        load.tile = rest - load.h * load.tiles();
+    }
+    Cursor<TILE> at = load;                                        // the tile that is computed next
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStageBytes);
+    uint64_t to_load = t1 - t0;
+
+    // one warp's rows of the tile at `load` into a stage; rows behind the sequence's end are zeros and read nothing
+    auto issue = [&](uint32_t stage) {
+        if (to_load) {
+            --to_load;
+            uint32_t row = kNoRow;
+            const uint32_t r = load.tile * TILE + warp * KEYS + lane;
+            if (lane < KEYS && r < load.n) row = c.row(load.b, load.h, r);
+            const uint32_t base = ring + stage * kStageBytes;
+#pragma unroll
+            for (int j = 0; j < KEYS * CH / 32; ++j) {
+                const uint32_t i = j * 32 + lane, rr = i / CH, ch = i % CH;
+                const uint32_t ri = __shfl_sync(0xFFFFFFFFu, row, rr);
+                const bool live = ri != kNoRow;
+                const size_t off = (size_t)(live ? ri : 0u) * D + ch * 8;
+                const uint32_t dst = base + rr * (D * 2) + ((ch ^ (rr & 7)) << 4);
+                cp16(dst, c.k + off, live);
+                cp16(dst + kStageBytes / 2, c.v + off, live);
+            }
+            load.next(c);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    uint32_t qf[NT][D / 16][2];
+    float acc[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) issue(s);
+
+    uint32_t stage = 0;
+    bool fresh = true;                                             // the next tile begins a segment
+    uint32_t seg_first = 0;
+    for (uint64_t t = t0; t < t1; ++t) {
+        if (fresh) {
+            fresh = false;
+            seg_first = at.tile;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t head = nt * 8 + g;
+                const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + ((size_t)at.b * hq + at.h * group + (head < group ? head : 0)) * D);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    qf[nt][kk][0] = head < group ? qr[kk * 8 + t4] : 0u;
+                    qf[nt][kk][1] = head < group ? qr[kk * 8 + 4 + t4] : 0u;
+                    for (int e = 0; e < 4; ++e) acc[nt][kk][e] = 0.0f;
+                }
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.0f;
+            }
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();
+        const uint32_t kbase = ring + stage * kStageBytes, vbase = kbase + kStageBytes / 2;
+        const uint32_t r0 = at.tile * TILE + warp * KEYS;
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+            if (r0 + sub * 16 >= at.n) break;
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                // keys on M: lanes 0-7 / 8-15 address keys 0-7 / 8-15 of the first 8 elements, 16-31 the same of the next 8
+                uint32_t a[4];
+                const uint32_t row = sub * 16 + (lane & 15), ch = kk * 2 + (lane >> 4);
+                ldsm_x4(kbase + row * (D * 2) + ((ch ^ (row & 7)) << 4), a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(s[nt], a, qf[nt][kk][0], qf[nt][kk][1]);
+            }
+            // thread: keys g, g + 8 (rows of s), heads 2 t4, 2 t4 + 1 of each n-tile
+            const uint32_t key = r0 + sub * 16 + g;
+            const bool live0 = key < at.n, live1 = key + 8 < at.n;
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[nt][e] = live0 ? __fmul_rn(s[nt][e], scale_log2) : -INFINITY;
+                    s[nt][2 + e] = live1 ? __fmul_rn(s[nt][2 + e], scale_log2) : -INFINITY;
+                    raise |= s[nt][e] > __fadd_rn(m[nt][e], kLazy) || s[nt][2 + e] > __fadd_rn(m[nt][e], kLazy);
+                    if (WEIGHTS) {
+                        const uint32_t head = nt * 8 + 2 * t4 + e;
+                        if (head < group) {
+                            float* dst = scores + ((size_t)at.b * hq + at.h * group + head) * c.cap();
+                            if (live0) dst[key] = s[nt][e];
+                            if (live1) dst[key + 8] = s[nt][2 + e];
+                        }
+                    }
+                }
+            }
+            if (__any_sync(0xFFFFFFFFu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+                        top = fmaxf(m[nt][e], top);
+                        const float f = top == m[nt][e] ? 1.0f : ex2(__fsub_rn(m[nt][e], top));
+                        m[nt][e] = top;
+                        l[nt][e] = __fmul_rn(l[nt][e], f);
+#pragma unroll
+                        for (int mt = 0; mt < D / 16; ++mt) {
+                            acc[nt][mt][e] = __fmul_rn(acc[nt][mt][e], f);
+                            acc[nt][mt][2 + e] = __fmul_rn(acc[nt][mt][2 + e], f);
+                        }
+                    }
+                }
+            }
+            uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                // a maximum of -inf (nothing but -inf so far) must not turn -inf - -inf into a NaN
+                const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+                const float p00 = ex2(__fsub_rn(s[nt][0], b0)), p01 = ex2(__fsub_rn(s[nt][1], b1));
+                const float p10 = ex2(__fsub_rn(s[nt][2], b0)), p11 = ex2(__fsub_rn(s[nt][3], b1));
+                l[nt][0] = __fadd_rn(l[nt][0], __fadd_rn(p00, p10));
+                l[nt][1] = __fadd_rn(l[nt][1], __fadd_rn(p01, p11));
+                const __nv_bfloat162 h0 = __floats2bfloat162_rn(p00, p01), h1 = __floats2bfloat162_rn(p10, p11);
+                const __nv_bfloat162 e0 = __floats2bfloat162_rn(__fsub_rn(p00, __low2float(h0)), __fsub_rn(p01, __high2float(h0)));
+                const __nv_bfloat162 e1 = __floats2bfloat162_rn(__fsub_rn(p10, __low2float(h1)), __fsub_rn(p11, __high2float(h1)));
+                hi[nt][0] = transpose8(*reinterpret_cast<const uint32_t*>(&h0));
+                hi[nt][1] = transpose8(*reinterpret_cast<const uint32_t*>(&h1));
+                lo[nt][0] = transpose8(*reinterpret_cast<const uint32_t*>(&e0));
+                lo[nt][1] = transpose8(*reinterpret_cast<const uint32_t*>(&e1));
+            }
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) {
+                // head dimension on M, keys on K: lanes 0-7 keys 0-7 of d 0-7, 8-15 keys 0-7 of d 8-15, 16-31 the same of keys 8-15
+                uint32_t a[4];
+                const uint32_t row = sub * 16 + (lane & 7) + ((lane >> 4) << 3), ch = mt * 2 + ((lane >> 3) & 1);
+                ldsm_x4_trans(vbase + row * (D * 2) + ((ch ^ (row & 7)) << 4), a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma(acc[nt][mt], a, hi[nt][0], hi[nt][1]);
+                    mma(acc[nt][mt], a, lo[nt][0], lo[nt][1]);
+                }
+            }
+        }
+        __syncwarp();
+        issue(stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+
+        const uint32_t unit_tiles = at.tiles(), b = at.b, h = at.h, tile = at.tile;
+        at.next(c);
+        if (at.tile != 0 && t + 1 < t1) continue;
+        // ---- the segment [seg_first, tile] of unit (b, h) is done: join the warps
+        fresh = true;
+        const bool whole = seg_first == 0 && tile + 1 == unit_tiles;
+        const uint32_t slot = cta * 2 + (seg_first == 0 ? 1u : 0u);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) l[nt][e] = __fadd_rn(l[nt][e], __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], off));
+                float* dst = merge + (warp * 8 + 2 * t4 + e) * S::kPitch + g;
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt) {
+                    dst[mt * 16] = acc[nt][mt][e];
+                    dst[mt * 16 + 8] = acc[nt][mt][2 + e];
+                }
+                if (g == 0) merge_ml[warp * 8 + 2 * t4 + e] = make_float2(m[nt][e], l[nt][e]);
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < 8 * D; i += kThreads) {
+                const uint32_t j = i / D, d = i % D, head = nt * 8 + j;
+                if (head >= group) break;
+                float M = merge_ml[j].x;
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, merge_ml[w * 8 + j].x);
+                float L = 0.0f, O = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 ml = merge_ml[w * 8 + j];
+                    const float f = ml.x == M ? 1.0f : ex2(__fsub_rn(ml.x, M));
+                    L = __fmaf_rn(ml.y, f, L);
+                    O = __fmaf_rn(merge[(w * 8 + j) * S::kPitch + d], f, O);
+                }
+                const size_t out_head = (size_t)b * hq + h * group + head;
+                if (whole) {
+                    o[out_head * D + d] = __float2bfloat16_rn(L == 0.0f ? 0.0f : __fdiv_rn(O, L));
+                    if (WEIGHTS && d == 0) stats[out_head] = make_float2(M, L);
+                } else {
+                    part.o[((size_t)slot * group + head) * D + d] = O;
+                    if (d == 0) part.ml[slot * 16 + head] = make_float2(M, L);
+                }
+            }
+            __syncthreads();
+        }
+        if (t + 1 == t1 && tid == 0)
+            part.first[cta] = !whole && seg_first == 0 ? make_uint4(1, b * c.hkv + h, unit_tiles - (tile + 1), 0) : make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Joins the parts of a unit that was cut: CTA c does it for the unit that CTA c of the first launch began and did not finish.
+// `tiles_left` tiles of it lie in the CTAs behind, which hold the same numbers of tiles the first launch computed.
+template <int D>
+__global__ void __launch_bounds__(kThreads) attn_decode_paged_join_kernel(View c, __nv_bfloat16* __restrict__ o, uint32_t hq, Partials part,
+                                                                          float2* __restrict__ stats) {
+    __shared__ uint64_t sums[kWarps];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t cta = blockIdx.x, C = gridDim.x, tid = threadIdx.x, group = hq / c.hkv;
+    const uint4 f = part.first[cta];
+    if (f.x == 0) return;
+    const uint64_t total = count_tiles<Shape<D>::kTile>(c, sums) * c.hkv;
+    const uint64_t n_cta = total < C ? total : C;
+    const uint64_t stop = (cta + 1) * total / n_cta + f.z;               // first tile behind the unit
+    const uint32_t last = (uint32_t)((stop * n_cta + total - 1) / total - 1);     // the CTA that holds tile stop - 1
+    const uint32_t b = f.y / c.hkv, h = f.y % c.hkv;
+    for (uint32_t i = tid; i < group * D; i += kThreads) {
+        const uint32_t head = i / D, d = i % D;
+        float M = part.ml[(cta * 2 + 1) * 16 + head].x;
+        for (uint32_t s = cta + 1; s <= last; ++s) M = fmaxf(M, part.ml[s * 2 * 16 + head].x);
+        float L = 0.0f, O = 0.0f;
+        for (uint32_t s = cta; s <= last; ++s) {
+            const uint32_t slot = s * 2 + (s == cta ? 1u : 0u);
+            const float2 ml = part.ml[slot * 16 + head];
+            const float w = ml.x == M ? 1.0f : ex2(__fsub_rn(ml.x, M));
+            L = __fmaf_rn(ml.y, w, L);
+            O = __fmaf_rn(part.o[((size_t)slot * group + head) * D + d], w, O);
+        }
+        const size_t out_head = (size_t)b * hq + h * group + head;
+        o[out_head * D + d] = __float2bfloat16_rn(L == 0.0f ? 0.0f : __fdiv_rn(O, L));
+        if (stats && d == 0) stats[out_head] = make_float2(M, L);
+    }
+}
+
+// weights_out[j] = weights_in[j] + sum over the group's heads, in ascending order, of exp2(s_j - M) / L
+__global__ void __launch_bounds__(256) attn_decode_paged_weights_kernel(View c, uint32_t hq, const float* __restrict__ scores, const float2* __restrict__ stats,
+                                                                        const float* weights_in, float* weights_out) {
+    __shared__ float s_m[16], s_r[16];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t unit = blockIdx.y, b = unit / c.hkv, group = hq / c.hkv, tid = threadIdx.x;
+    const uint32_t n = c.length(b), j0 = blockIdx.x * 1024;
+    if (j0 >= n) return;
+    if (tid < group) {
+        const float2 ml = stats[(size_t)unit * group + tid];
+        s_m[tid] = ml.x == -INFINITY ? 0.0f : ml.x;
+        s_r[tid] = ml.y == 0.0f ? 0.0f : __frcp_rn(ml.y);
+    }
+    __syncthreads();
+    for (uint32_t j = j0 + tid; j < min(j0 + 1024, n); j += 256) {
+        float w = 0.0f;
+        for (uint32_t i = 0; i < group; ++i) w = __fmaf_rn(ex2(__fsub_rn(scores[((size_t)unit * group + i) * c.cap() + j], s_m[i])), s_r[i], w);
+        const size_t at = (size_t)unit * c.cap() + j;
+        weights_out[at] = weights_in ? __fadd_rn(weights_in[at], w) : w;
+    }
+}
+
+// ---------------------------------------------------------------- host side
+struct Plan {
+    uint32_t ctas;
+    uint64_t first, ml, o, stats, scores, bytes;       // byte offsets into the workspace
+};
+static Plan plan_for(const View& c, uint64_t d, uint64_t hq, bool weights) {
+    Plan p = {};
+    int sms = tls().sm_count > 0 ? tls().sm_count : 148;
+    const uint64_t tile = d == 128 ? Shape<128>::kTile : Shape<64>::kTile;
+    const uint64_t most = (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), tile);      // tiles when every sequence is full
+    p.ctas = (uint32_t)(most < (uint64_t)sms * kCtasPerSm ? most : (uint64_t)sms * kCtasPerSm);
+    const uint64_t group = hq / c.hkv;
+    auto take = [&](uint64_t bytes) { const uint64_t at = p.bytes; p.bytes += (bytes + 255) & ~255ull; return at; };
+    p.first = take(p.ctas * sizeof(uint4));
+    p.ml = take((uint64_t)p.ctas * 2 * 16 * sizeof(float2));
+    p.o = take((uint64_t)p.ctas * 2 * group * d * sizeof(float));
+    if (weights) {
+        p.stats = take((uint64_t)c.n_seqs * hq * sizeof(float2));
+        p.scores = take((uint64_t)c.n_seqs * hq * c.cap() * sizeof(float));
+    }
+    return p;
+}
+static catena_status_t check_heads(const View& c, uint64_t hq) {
+    if (hq == 0 || hq % c.hkv || hq / c.hkv > 16) return fail(CATENA_E_UNSUPPORTED, "attn_decode_paged: heads must be a multiple (<= 16) of kv heads");
+    return CATENA_OK;
+}
+
+template <int D, int NT, bool WEIGHTS>
+static catena_status_t launch_attention(const View& c, const Plan& p, const void* q, void* o, uint64_t hq, float scale, uint8_t* ws) {
+    auto kernel = attn_decode_paged_kernel<D, NT, WEIGHTS>;
+    CATENA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem));
+    const Partials part = {(uint4*)(ws + p.first), (float2*)(ws + p.ml), (float*)(ws + p.o)};
+    float2* stats = WEIGHTS ? (float2*)(ws + p.stats) : nullptr;
+    CATENA_TRY(launch("attn_decode_paged_kernel", kernel, dim3(p.ctas), dim3(kThreads), Shape<D>::kSmem, c, (const __nv_bfloat16*)q,
+                      (__nv_bfloat16*)o, (uint32_t)hq, scale * 1.44269504088896340736f, part, WEIGHTS ? (float*)(ws + p.scores) : nullptr, stats));
+    return launch("attn_decode_paged_join_kernel", attn_decode_paged_join_kernel<D>, dim3(p.ctas), dim3(kThreads), 0, c, (__nv_bfloat16*)o,
+                  (uint32_t)hq, part, stats);
+}
+
+}  // namespace paged
+
+using namespace paged;
+
+extern "C" {
+
+uint64_t catena_b200_attn_decode_paged_workspace_bytes(const catena_paged_cache_t* cache, uint64_t n_heads, int weights) {
+    View c;
+    if (check_cache(cache, "attn_decode_paged: null cache", &c) != CATENA_OK || check_heads(c, n_heads) != CATENA_OK) return 0;
+    return plan_for(c, cache->head_dim, n_heads, weights != 0).bytes;
+}
+
+catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache_t* cache, const void* q, void* o, uint64_t n_heads, float scale,
+                                                        const float* weights_in, float* weights_out, void* workspace, uint64_t workspace_bytes) {
+    View c;
+    CATENA_TRY(check_cache(cache, "attn_decode_paged: null cache", &c));
+    CATENA_TRY(check_heads(c, n_heads));
+    if (!c.n_seqs) return CATENA_OK;
+    if (!q || !o || !workspace || (weights_in && !weights_out)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: null argument");
+    if (!aligned16(q) || !aligned16(o) || !aligned4(weights_in) || !aligned4(weights_out) || ((uintptr_t)workspace & 255))
+        return fail(CATENA_E_BAD_ARG, "attn_decode_paged: q and o must be 16-byte aligned, the workspace 256-byte");
+    if (scale - scale != 0.0f) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite");
+    if (weights_out && (uint64_t)c.n_seqs * c.hkv > 65535) return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: weights of more than 65535 (sequence, kv head) pairs");
+    CATENA_TRY(begin(&c.err));
+    const Plan p = plan_for(c, cache->head_dim, n_heads, weights_out != nullptr);
+    if (workspace_bytes < p.bytes) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: workspace too small");
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const bool wide = n_heads / c.hkv > 8, w = weights_out != nullptr;
+    using Fn = catena_status_t (*)(const View&, const Plan&, const void*, void*, uint64_t, float, uint8_t*);
+    static const Fn table[2][2][2] = {{{launch_attention<64, 1, false>, launch_attention<64, 1, true>}, {launch_attention<64, 2, false>, launch_attention<64, 2, true>}},
+                                      {{launch_attention<128, 1, false>, launch_attention<128, 1, true>}, {launch_attention<128, 2, false>, launch_attention<128, 2, true>}}};
+    CATENA_TRY(table[cache->head_dim == 128][wide][w](c, p, q, o, n_heads, scale, ws));
+    if (w) {
+        const dim3 grid((unsigned)ceil_div_u64(c.cap(), 1024), c.n_seqs * c.hkv);
+        CATENA_TRY(launch("attn_decode_paged_weights_kernel", attn_decode_paged_weights_kernel, grid, dim3(256), 0, c, (uint32_t)n_heads,
+                          (const float*)(ws + p.scores), (const float2*)(ws + p.stats), weights_in, weights_out));
+    }
+    return end();
+}
+
+}  // extern "C"
+
+}  // namespace catena

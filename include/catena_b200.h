@@ -402,6 +402,81 @@ catena_status_t catena_b200_add_bf16_into(const void* x, const void* y, void* ou
 catena_status_t catena_b200_linear_bf16_into(const void* x, const void* w, const void* residual, void* y, uint64_t m, uint64_t n,
                                              uint64_t k);
 
+/* ---- key/value cache in pages, for serving ------------------------------------------------------------------
+ * No counterpart in the reference.  The contiguous caches above give every sequence max_len rows and put all sequences at one
+ * position; here sequences have lengths of their own and take memory page by page.  Row r of sequence b lies in page
+ * table[b][r / page_size] of the pools, at row r % page_size of it, [page][kv head][row][head_dim]; any page_size, head_dim 64 or
+ * 128, page ids in any order, pages may be shared by sequences for reading.  All pointers are DEVICE pointers, q / k / v / o are
+ * bf16, table, lengths, positions and parents int32; the struct itself is host memory and read during the call only.
+ * The calls only enqueue (and, in blocking mode, wait), so a graph can capture them in non-blocking mode on any but the legacy
+ * stream, after one call of this thread on this device; a graph that is replayed reads lengths and tables anew.  Two calls
+ * that may overlap on the device must not share a workspace, an output or a page that one of them writes.
+ * Page ids, lengths, positions and parents are checked on the device: what is out of range is skipped, never read or written, and
+ * the call returns CATENA_E_ASSERT (in non-blocking mode: the next catena_b200_check_device_errors); the outputs of the sequences
+ * concerned are then undefined. */
+typedef struct catena_paged_cache_t {
+    void* k_pages;           /* [n_pages, n_kv_heads, page_size, head_dim], 16-byte aligned */
+    void* v_pages;
+    const int32_t* table;    /* [n_seqs, max_pages]; entries behind a sequence's last row are not read */
+    const int32_t* lengths;  /* [n_seqs] rows of each sequence, 0 .. max_pages * page_size */
+    uint64_t n_pages, page_size, n_seqs, max_pages, n_kv_heads, head_dim;
+} catena_paged_cache_t;
+/* angles [count][head_dim / 2] of (cos, sin) pairs for positions pos0 .. pos0 + count - 1, with the functions of
+ * catena_b200_rope_append_bf16_into (the same bits for head_dim 128) */
+catena_status_t catena_b200_rope_angles_f32_into(float base, uint64_t pos0, uint64_t count, uint64_t head_dim, void* angles);
+/* Rotation and append of ragged tokens.  Tokens token_start[b] .. token_start[b + 1] - 1 (ascending, [n_seqs + 1]; NULL: one token
+ * per sequence) are the LAST rows of sequence b: lengths counts them already, and their pages are in the table.  qkv [tokens]
+ * rows of (n_heads + 2 n_kv_heads) * head_dim elements, qkv_pitch elements apart (a multiple of 8).  A token's position is
+ * positions[b] (NULL: lengths[b] minus the new tokens) plus its number within the sequence's new tokens; after an eviction positions
+ * go on counting where lengths do not.  angles [n_angles][head_dim / 2] (cos, sin), from catena_b200_rope_angles_f32_into or of
+ * the caller's own scaling.  Writes the rotated queries to q_out [tokens, n_heads, head_dim], rotated keys and plain values to the pages.
+ * Tokens before token_start[0] and behind token_start[n_seqs] belong to nobody and their rows of q_out stay as they were. */
+catena_status_t catena_b200_rope_append_paged_bf16_into(const catena_paged_cache_t* cache, const void* qkv, uint64_t qkv_pitch,
+                                                        const int32_t* token_start, uint64_t tokens, const int32_t* positions,
+                                                        const void* angles, uint64_t n_angles, uint64_t n_heads, void* q_out);
+/* Attention of one token per sequence over all its rows: q, o [n_seqs, n_heads, head_dim]; n_heads a multiple of n_kv_heads, at
+ * most 16 times.  o = softmax(scale q k^T) v with the true exponential (not math.exp-approx); probabilities, sums and the running
+ * maximum are f32.  A sequence without rows, or whose scores are all -inf, gives zeros.  With weights_out [n_seqs, n_kv_heads,
+ * max_pages * page_size] f32: weights_out = weights_in + the attention each row gets, summed over the query heads of its kv head
+ * (weights_in NULL: zeros; both may be one buffer); elements behind a sequence's rows stay as they were.
+ * Equal calls give equal bits; the split of a sequence depends on the other lengths of the call, so its last bits may, too.
+ * The workspace is caller-owned, 256-byte aligned, and needs no preparation. */
+uint64_t catena_b200_attn_decode_paged_workspace_bytes(const catena_paged_cache_t* cache, uint64_t n_heads, int weights);
+catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache_t* cache, const void* q, void* o, uint64_t n_heads, float scale,
+                                                        const float* weights_in, float* weights_out, void* workspace, uint64_t workspace_bytes);
+/* Eviction by accumulated attention weight.  Per sequence and kv head min(length, budget) rows stay: the `recent` last ones and, of the
+ * others, those of the greatest weight (ties: the lowest row; NaN counts as -inf).  They go in their order to rows 0, 1, ... of
+ * the pages of table_out [n_seqs, max_pages_out] in the same pools, which must be other pages than those of cache->table (that
+ * may be shared with other sequences: they are only read).  lengths_out [n_seqs]; weights_out [n_seqs, n_kv_heads, max_pages_out *
+ * page_size]: the weights of the rows that stay, zeros behind; kept (may be NULL) [n_seqs, n_kv_heads, budget]: the rows' numbers, elements
+ * behind the last one stay as they were.  Keys keep the rotation of the position they were appended at. */
+uint64_t catena_b200_kv_evict_paged_workspace_bytes(const catena_paged_cache_t* cache, uint64_t budget);
+catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t* cache, const float* weights, uint64_t budget, uint64_t recent,
+                                                     const int32_t* table_out, uint64_t max_pages_out, int32_t* lengths_out,
+                                                     float* weights_out, int32_t* kept, void* workspace, uint64_t workspace_bytes);
+
+/* ---- beam search ----------------------------------------------------------------------------------------------
+ * Selection: of the beams x vocabulary continuations of each request the k best by scores[request][beam] + log softmax(logits), in
+ * descending order (ties: the lowest beam, then the greater logit, then the lowest token); logits [batch * beams] rows of `vocab`,
+ * `pitch` elements apart, bf16 or f32.  Candidates of one beam are ordered by their logits, those of different beams by totals in f64.  A logit of -inf or NaN gives a total
+ * of -inf (chosen only when nothing else is left), +inf counts as the greatest finite f32; a NaN total counts as -inf.  Writes
+ * out_scores / out_parents (beam within the request) / out_tokens [batch, k]; at most 64 beams and k <= 64.  The workspace is caller-owned, 256-byte
+ * aligned. */
+uint64_t catena_b200_beam_select_workspace_bytes(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k);
+catena_status_t catena_b200_beam_select_f32_into(const float* logits, uint64_t pitch, const float* scores, uint64_t batch, uint64_t beams,
+                                                 uint64_t vocab, uint64_t k, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                                                 void* workspace, uint64_t workspace_bytes);
+catena_status_t catena_b200_beam_select_bf16_into(const void* logits, uint64_t pitch, const float* scores, uint64_t batch, uint64_t beams,
+                                                  uint64_t vocab, uint64_t k, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                                                  void* workspace, uint64_t workspace_bytes);
+/* Reordering of the states: sequence s = request * beams + i of the output takes over sequence request * beams + parents[s].  Its full
+ * pages are shared (table_out names them), the page that is still being filled is copied to page fresh_pages[s] (of the same pools; used by nothing
+ * else), entries of table_out behind it stay as they were.  lengths_out [n_seqs]; weights and weights_out (both or neither, [n_seqs, n_kv_heads,
+ * max_pages * page_size]): the parent's, zeros behind its rows.  The outputs are other buffers than the inputs. */
+catena_status_t catena_b200_beam_reorder_paged_bf16_into(const catena_paged_cache_t* cache, const int32_t* parents, uint64_t beams,
+                                                         const int32_t* fresh_pages, int32_t* table_out, int32_t* lengths_out,
+                                                         const float* weights, float* weights_out);
+
 /* test hook: cap the persistent grid of the tensor-core GEMM (0 = one CTA per SM); results must not
  * change with it.  No counterpart in the reference. */
 void catena_b200_debug_set_cta_limit(int limit);
@@ -446,7 +521,8 @@ catena_status_t catena_b200_debug_packed_f32x2_check(uint64_t out[3]);
  * such a launch is undefined; the library stays usable.  No counterpart in the reference. */
 void catena_b200_debug_set_wait_limit_ns(uint64_t ns);
 void catena_b200_debug_stall_next(int family, uint32_t value);
-/* after non-blocking launches: reports (and clears) a device-side bounded-wait expiry or what a map program ran into */
+/* after non-blocking launches: reports (and clears) a device-side bounded-wait expiry, what a map program ran into, or an index
+ * out of range that a kernel over a paged cache met */
 catena_status_t catena_b200_check_device_errors(void);
 
 #ifdef __cplusplus
