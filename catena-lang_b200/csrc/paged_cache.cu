@@ -1,10 +1,12 @@
 // A key/value cache in pages: rotation and append of ragged tokens, eviction by accumulated attention weight, and the hand-over
 // of pages between the beams of a beam search.  (The attention that reads the pages: attn_decode_paged.cu.)
 // The reference has no cache; layouts follow this library's contiguous caches [batch, n_kv_heads, rows, head_dim].
-#include <string.h>
+#include <cooperative_groups.h>
 
 #include "catena_math.cuh"
 #include "paged.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace catena {
 namespace paged {
@@ -175,18 +177,29 @@ __global__ void __launch_bounds__(128) rope_append_paged_kernel(View c, const __
 }
 
 // ---------------------------------------------------------------- eviction: which rows stay
-// One CTA per (sequence, kv head).  Rows 0 .. n - recent - 1 compete by weight for budget - recent places; the place's limit is
-// found by a radix select over the weights' order-preserving bits (11 + 11 + 10), ties at the limit go to the lowest rows.
-// A NaN counts as -inf and -0 as +0, so the order is total.
-constexpr int kSelThreads = 1024;
+// A cluster of CTAs per (sequence, kv head), each with a stretch of the rows, whose weights it keeps in shared memory as
+// order-preserving bits.  Rows 0 .. n - recent - 1 compete by weight for budget - recent places; the limit is found by a radix
+// select, 2048 bins between the least and the greatest weight (weights spread over few octaves, so bins cut from the top bits
+// would hold thousands each, and the updates of their counters queue up), every CTA adding up all CTAs' bins for itself.  One pass
+// usually leaves a bin of at most 256 rows, which are ranked by comparing them with each other; ties at the limit go to the lowest rows.
+// A NaN counts as -inf and -0 as +0, so the order is total.  What stays is then written in order: every warp counts in its part
+// of the stretch and writes once it knows how many stay before it.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kBinsPer = kBins / kSelThreads;
+constexpr uint32_t kRanked = 256;
+constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kSelRoom = 49152;                   // weights a CTA can hold (192 KB)
+constexpr uint32_t kSelAlone = 116 * 1024;             // more than half of an SM's shared memory
 
 __device__ __forceinline__ uint32_t order_bits(float w) {
     if (w != w) return 0x007FFFFFu;                    // -inf
     const uint32_t u = __float_as_uint(w + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// exclusive prefix sum over the CTA of one value per thread; the total in *total
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+// exclusive prefix sum over the CTA of one value per thread
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t x = v;
 #pragma unroll
@@ -196,95 +209,191 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
     }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t s = warp_sums[lane];
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, s, off);
-            if (lane >= (uint32_t)off) s += y;
-        }
-        warp_sums[lane] = s;
-    }
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? warp_sums[lane] : 0u);
     __syncthreads();
-    const uint32_t base = warp ? warp_sums[warp - 1] : 0;
-    *total = warp_sums[31];
-    __syncthreads();
-    return base + x - v;
+    return before + x - v;
 }
 
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const float* __restrict__ weights, uint32_t budget, uint32_t recent,
                                                                    int32_t* __restrict__ lengths_out, float* __restrict__ weights_out,
-                                                                   uint32_t cap_out, int32_t* __restrict__ kept, int32_t* __restrict__ rows_ws) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t warp_sums[32];
-    __shared__ uint32_t s_digit, s_left;
+                                                                   uint32_t cap_out, int32_t* __restrict__ kept, int32_t* __restrict__ rows_ws,
+                                                                   uint32_t room) {
+    extern __shared__ uint32_t sel_smem[];             // [room] bits of the stretch's weights, [room / 32] who stays
+    __shared__ __align__(8) uint32_t hist[kBins];
+    __shared__ uint64_t cand[kRanked], all[kRanked];
+    __shared__ uint32_t warp_sums[32], s_lo, s_hi, s_digit, s_left, s_count, s_n, s_equal, s_stay;
+    __shared__ uint64_t s_limit;
     pdl_trigger();
     pdl_wait();
-    const uint32_t unit = blockIdx.x, b = unit / c.hkv, tid = threadIdx.x;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t unit = blockIdx.x / ctas, b = unit / c.hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t n = c.length(b);
     const uint32_t stay = min(n, budget);
     const float* w = weights + (size_t)unit * c.cap();
     float* w_out = weights_out + (size_t)unit * cap_out;
     int32_t* rows = rows_ws + (size_t)unit * budget;
     int32_t* kept_row = kept ? kept + (size_t)unit * budget : nullptr;
-    if (unit % c.hkv == 0 && tid == 0) lengths_out[b] = (int32_t)stay;
+    if (unit % c.hkv == 0 && rank == 0 && tid == 0) lengths_out[b] = (int32_t)stay;
+    for (uint32_t i = stay + rank * kSelThreads + tid; i < cap_out; i += ctas * kSelThreads) w_out[i] = 0.0f;
     if (n <= budget) {
-        for (uint32_t i = tid; i < n; i += kSelThreads) {
+        for (uint32_t i = rank * kSelThreads + tid; i < n; i += ctas * kSelThreads) {
             rows[i] = (int32_t)i;
             if (kept_row) kept_row[i] = (int32_t)i;
             w_out[i] = w[i];
         }
-    } else {
-        const uint32_t m = n - recent, want = budget - recent;     // want < m
-        uint32_t limit = 0xFFFFFFFFu, left = 0;                    // rows above `limit` stay, and the first `left` that equal it
-        if (want) {
-            uint32_t prefix = 0, prefix_bits = 0;
-            left = want;
-            for (int pass = 0; pass < 3; ++pass) {
-                const uint32_t bits = pass == 2 ? 10 : 11, shift = 32 - prefix_bits - bits;
-                for (uint32_t i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-                __syncthreads();
-                for (uint32_t i = tid; i < m; i += kSelThreads) {
-                    const uint32_t u = order_bits(w[i]);
-                    if (prefix_bits == 0 || (u >> (32 - prefix_bits)) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1u);
-                }
-                __syncthreads();
-                // the digit whose bin holds the left-th largest: suffix sums, two bins per thread, largest digit first
-                const uint32_t nb = 1u << bits, d1 = nb - 1 - 2 * tid, d0 = nb - 2 - 2 * tid;
-                const bool mine = 2 * tid < nb;
-                const uint32_t h1 = mine ? hist[d1] : 0, h0 = mine ? hist[d0] : 0;
-                uint32_t total;
-                const uint32_t above = block_scan(h1 + h0, warp_sums, &total);
-                if (mine && above < left && left <= above + h1) { s_digit = d1; s_left = left - above; }
-                if (mine && above + h1 < left && left <= above + h1 + h0) { s_digit = d0; s_left = left - above - h1; }
-                __syncthreads();
-                left = s_left;
-                prefix = (prefix << bits) | s_digit;
-                prefix_bits += bits;
-                __syncthreads();
-            }
-            limit = prefix;
+        return;
+    }
+    const uint32_t m = n - recent, want = budget - recent;         // want < m
+    const uint32_t part = (n + ctas * kSelWarps * 32 - 1) / (ctas * kSelWarps * 32) * 32;      // rows of a warp
+    const uint32_t r0 = min(n, rank * kSelWarps * part), r1 = min(n, r0 + kSelWarps * part), c1 = min(r1, max(m, r0));
+    uint32_t* bits = sel_smem;
+    uint32_t* words = sel_smem + room;
+    const bool held = kSelWarps * part <= room;                    // else the weights are read again in every pass
+    auto key = [&](uint32_t i) { return held ? bits[i - r0] : order_bits(w[i]); };
+    // a value of every CTA of the cluster, lane q that of CTA q (0 behind the last)
+    auto of_all = [&](uint32_t* mine) { return lane < ctas ? *cluster.map_shared_rank(mine, lane) : 0u; };
+
+    if (tid == 0) { s_lo = 0xFFFFFFFFu; s_hi = 0; s_n = s_equal = 0; }
+    for (uint32_t i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    {
+        uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll 4
+        for (uint32_t i = r0 + tid; i < r1; i += kSelThreads) {
+            const uint32_t u = order_bits(w[i]);
+            if (held) bits[i - r0] = u;
+            if (i < m) { lo = min(lo, u); hi = max(hi, u); }
         }
-        uint32_t out0 = 0, eq0 = 0;                                // rows and ties taken by earlier blocks of rows
-        for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
-            const uint32_t i = i0 + tid;
-            uint32_t u = 0;
-            if (want && i < m) u = order_bits(w[i]);
-            const uint32_t eq = want && i < m && u == limit ? 1u : 0u;
-            uint32_t n_eq, n_out;
-            const uint32_t eq_before = eq0 + block_scan(eq, warp_sums, &n_eq);
-            const bool keep = (i < n && i >= m) || (want && i < m && (u > limit || (eq && eq_before < left)));
-            const uint32_t at = out0 + block_scan(keep ? 1u : 0u, warp_sums, &n_out);
-            if (keep) {
-                rows[at] = (int32_t)i;
-                if (kept_row) kept_row[at] = (int32_t)i;
-                w_out[at] = w[i];
-            }
-            eq0 += n_eq;
-            out0 += n_out;
+        lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+        hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+        if (lane == 0) {
+            atomicMin(&s_lo, lo);
+            atomicMax(&s_hi, hi);
         }
     }
-    for (uint32_t i = stay + tid; i < cap_out; i += kSelThreads) w_out[i] = 0.0f;
+    uint64_t limit = ~0ull;                                        // a row stays when (bits, lowest row first) reaches it
+    if (want) {
+        cluster.sync();
+        const uint32_t his = of_all(&s_hi), los = lane < ctas ? *cluster.map_shared_rank(&s_lo, lane) : 0xFFFFFFFFu;
+        uint32_t lo = __reduce_min_sync(0xFFFFFFFFu, los);
+        uint32_t span = __reduce_max_sync(0xFFFFFFFFu, his) - lo, left = want, count;      // keys lo .. lo + span; the left-th greatest
+        int shift = max(0, 21 - __clz(span));                      // span >> shift < 2048 (clz(0) is 32)
+        while (true) {
+#pragma unroll 4
+            for (uint32_t i = r0 + tid; i < c1; i += kSelThreads) {
+                const uint32_t d = key(i) - lo;
+                if (d <= span) atomicAdd(&hist[d >> shift], 1u);
+            }
+            cluster.sync();
+            // the bin of the left-th greatest: sums from the top
+            uint32_t h[kBinsPer], sum = 0;
+            const uint32_t top = kBins - kBinsPer * (tid + 1);
+#pragma unroll
+            for (uint32_t e = 0; e < kBinsPer; ++e) h[e] = 0;
+            for (uint32_t q = 0; q < ctas; ++q) {
+                const uint2* bins = cluster.map_shared_rank(reinterpret_cast<uint2*>(hist + top), q);
+#pragma unroll
+                for (uint32_t e = 0; e < kBinsPer; e += 2) {
+                    const uint2 v = bins[kBinsPer / 2 - 1 - e / 2];
+                    h[e] += v.y;
+                    h[e + 1] += v.x;
+                }
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < kBinsPer; ++e) sum += h[e];
+            uint32_t above = block_scan(sum, warp_sums);
+#pragma unroll
+            for (uint32_t e = 0; e < kBinsPer; ++e) {
+                if (above < left && left <= above + h[e]) { s_digit = top + kBinsPer - 1 - e; s_left = left - above; s_count = h[e]; }
+                above += h[e];
+            }
+            __syncthreads();
+            lo += s_digit << shift;
+            span = (1u << shift) - 1;
+            left = s_left;
+            count = s_count;
+            if (count <= kRanked || shift == 0) break;
+            shift = max(0, shift - 11);
+            cluster.sync();                                        // everyone has read the bins
+            for (uint32_t i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+            __syncthreads();
+        }
+        if (count <= kRanked) {
+#pragma unroll 4
+            for (uint32_t i = r0 + tid; i < c1; i += kSelThreads) {
+                const uint32_t u = key(i);
+                if (u - lo <= span) cand[atomicAdd(&s_n, 1u)] = (uint64_t)u << 32 | (uint32_t)~i;
+            }
+            cluster.sync();
+            const uint32_t sizes = of_all(&s_n);
+            uint32_t at = 0;
+            for (uint32_t q = 0; q < ctas; ++q) {
+                const uint32_t size = __shfl_sync(0xFFFFFFFFu, sizes, q);
+                if (tid < size) all[at + tid] = cluster.map_shared_rank(cand, q)[tid];
+                at += size;
+            }
+            __syncthreads();
+            if (tid < count) {
+                const uint64_t mine = all[tid];
+                uint32_t before = 0;
+                for (uint32_t j = 0; j < count; ++j) before += all[j] > mine;
+                if (before == left - 1) s_limit = mine;
+            }
+        } else {
+            // more than 256 rows of one weight: the left-th lowest of them
+            uint32_t mine = 0;
+            const uint32_t i0 = r0 + warp * part;
+            for (uint32_t i = i0; i < i0 + part; i += 32) mine += __popc(__ballot_sync(0xFFFFFFFFu, i + lane < c1 && key(i + lane) == lo));
+            if (lane == 0) {
+                warp_sums[warp] = mine;
+                atomicAdd(&s_equal, mine);
+            }
+            cluster.sync();
+            const uint32_t equal = of_all(&s_equal);
+            uint32_t before = __reduce_add_sync(0xFFFFFFFFu, (lane < rank ? equal : 0u) + (lane < warp ? warp_sums[lane] : 0u));
+            if (before < left && left <= before + mine)
+                for (uint32_t i = i0; i < i0 + part; i += 32) {
+                    const bool eq = i + lane < c1 && key(i + lane) == lo;
+                    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, eq);
+                    if (eq && before + __popc(votes & ((1u << lane) - 1)) == left - 1)
+                        for (uint32_t q = 0; q < ctas; ++q) *cluster.map_shared_rank(&s_limit, q) = (uint64_t)lo << 32 | (uint32_t)~(i + lane);
+                    before += __popc(votes);
+                }
+            cluster.sync();
+        }
+        __syncthreads();
+        limit = s_limit;
+    }
+    __syncthreads();                                               // `bits` is complete, warp_sums of the tie search has been read
+    auto stays = [&](uint32_t i) { return i < r1 && (i >= m || ((uint64_t)key(i) << 32 | (uint32_t)~i) >= limit); };
+    const uint32_t i0 = r0 + warp * part;
+    uint32_t mine = 0;
+#pragma unroll 4
+    for (uint32_t i = i0; i < i0 + part; i += 32) {
+        const uint32_t votes = __ballot_sync(0xFFFFFFFFu, stays(i + lane));
+        if (held && lane == 0) words[(i - r0) / 32] = votes;
+        mine += __popc(votes);
+    }
+    if (lane == 0) warp_sums[warp] = mine;
+    __syncthreads();
+    uint32_t at = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? warp_sums[lane] : 0u);
+    if (warp == kSelWarps - 1 && lane == 0) s_stay = at + mine;
+    cluster.sync();
+    const uint32_t staying = of_all(&s_stay);
+    at += __reduce_add_sync(0xFFFFFFFFu, lane < rank ? staying : 0u);
+    cluster.sync();                                                // no CTA leaves while another reads from it
+#pragma unroll 4
+    for (uint32_t i = i0; i < i0 + part; i += 32) {
+        const uint32_t votes = held ? words[(i - r0) / 32] : __ballot_sync(0xFFFFFFFFu, stays(i + lane));
+        if (votes >> lane & 1) {
+            const uint32_t to = at + __popc(votes & ((1u << lane) - 1));
+            rows[to] = (int32_t)(i + lane);
+            if (kept_row) kept_row[to] = (int32_t)(i + lane);
+            w_out[to] = w[i + lane];
+        }
+        at += __popc(votes);
+    }
 }
 
 // ---------------------------------------------------------------- eviction: the rows that stay, into their new pages
@@ -293,23 +402,34 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(View c, const int32_t* 
                                                          const int32_t* __restrict__ table_out, uint32_t max_pages_out) {
     constexpr uint32_t kLanes = D / 8;                 // 16-byte pieces of a row
     constexpr uint32_t kRows = 256 / kLanes;           // rows of a CTA's step
+    constexpr int kSteps = 4;
     pdl_trigger();
     pdl_wait();
     const uint32_t unit = blockIdx.y, b = unit / c.hkv, h = unit % c.hkv;
     const uint32_t stay = min(c.length(b), budget);
-    const uint32_t piece = threadIdx.x % kLanes;
+    const uint32_t piece = threadIdx.x % kLanes, i0 = blockIdx.x * (kSteps * kRows) + threadIdx.x / kLanes;
+    if (i0 >= stay) return;
+    uint32_t src[kSteps], dst[kSteps];
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-        const uint32_t i = (blockIdx.x * 4 + u) * kRows + threadIdx.x / kLanes;
-        if (i >= stay) return;
-        const uint32_t src = c.row(b, h, (uint32_t)rows_ws[(size_t)unit * budget + i]);
-        const uint32_t dst = c.row(table_out, max_pages_out, b, h, i);
-        if (src == kNoRow || dst == kNoRow) continue;
-        const uint4 k = reinterpret_cast<const uint4*>(c.k)[(size_t)src * kLanes + piece];
-        const uint4 v = reinterpret_cast<const uint4*>(c.v)[(size_t)src * kLanes + piece];
-        reinterpret_cast<uint4*>(c.k)[(size_t)dst * kLanes + piece] = k;
-        reinterpret_cast<uint4*>(c.v)[(size_t)dst * kLanes + piece] = v;
+    for (int u = 0; u < kSteps; ++u) src[u] = i0 + u * kRows < stay ? (uint32_t)rows_ws[(size_t)unit * budget + i0 + u * kRows] : kNoRow;
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+        dst[u] = src[u] == kNoRow ? kNoRow : c.row(table_out, max_pages_out, b, h, i0 + u * kRows);
+        src[u] = dst[u] == kNoRow ? kNoRow : c.row(b, h, src[u]);
     }
+    uint4 k[kSteps], v[kSteps];
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+        if (src[u] != kNoRow) {
+            k[u] = reinterpret_cast<const uint4*>(c.k)[(size_t)src[u] * kLanes + piece];
+            v[u] = reinterpret_cast<const uint4*>(c.v)[(size_t)src[u] * kLanes + piece];
+        }
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+        if (src[u] != kNoRow) {
+            reinterpret_cast<uint4*>(c.k)[(size_t)dst[u] * kLanes + piece] = k[u];
+            reinterpret_cast<uint4*>(c.v)[(size_t)dst[u] * kLanes + piece] = v[u];
+        }
 }
 
 // ---------------------------------------------------------------- beams take over their parents' pages
@@ -430,8 +550,20 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     const uint64_t units = (uint64_t)c.n_seqs * c.hkv;
     if (units > 65535) return fail(CATENA_E_TOO_LARGE, "kv_evict_paged: more than 65535 (sequence, kv head) pairs");
     CATENA_TRY(begin(&c.err));
-    CATENA_TRY(launch("evict_select_kernel", evict_select_kernel, dim3((unsigned)units), dim3(kSelThreads), 0, c, weights, (uint32_t)budget,
-                      (uint32_t)recent, lengths_out, weights_out, (uint32_t)(max_pages_out * c.page_size), kept, (int32_t*)workspace));
+    // A CTA per 1024 rows that a sequence may have, up to eight and as long as every CTA has an SM of its own.  (Clusters of small
+    // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take SELTIME.)  The shared memory that keeps a second CTA
+    // off the SM is asked for whether it is filled or not.
+    const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148;
+    uint32_t ctas = 1;
+    while (ctas < kMaxCluster && c.cap() > 1024u * ctas && units * ctas * 2 <= sms) ctas *= 2;
+    const uint64_t stretch = ceil_div_u64(c.cap(), ctas * kSelWarps * 32) * (kSelWarps * 32);
+    const uint32_t room = stretch > kSelRoom ? 0u : (uint32_t)stretch;
+    size_t smem = (size_t)room * 4 + room / 8;
+    if (ctas > 1 && smem < kSelAlone) smem = kSelAlone;
+    if (smem > 32768) CATENA_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelRoom * 4 + kSelRoom / 8));
+    CATENA_TRY(launch_cluster("evict_select_kernel", evict_select_kernel, dim3((unsigned)units * ctas), dim3(kSelThreads), smem, ctas, c, weights,
+                              (uint32_t)budget, (uint32_t)recent, lengths_out, weights_out, (uint32_t)(max_pages_out * c.page_size), kept,
+                              (int32_t*)workspace, room));
     const uint64_t rows_per_cta = 4 * (256 / (cache->head_dim / 8));
     const dim3 grid((unsigned)ceil_div_u64(budget, rows_per_cta), (unsigned)units);
     CATENA_TRY(launch("evict_copy_kernel", cache->head_dim == 128 ? evict_copy_kernel<128> : evict_copy_kernel<64>, grid, dim3(256), 0, c,
