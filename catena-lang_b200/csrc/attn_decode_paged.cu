@@ -11,11 +11,13 @@
 // under the tensor rate; mma.sync on 16-row pieces feeds from a ring that each warp fills for itself with cp.async, and no warp
 // waits for another while it streams.
 //
-// Split: all (sequence, kv head) units' rows are cut into tiles of 64 (d = 128) or 128 (d = 64) keys, and CTA c of C takes tiles
-// [c T / C, (c + 1) T / C) of the T there are (C = T when there are fewer tiles than CTAs): every CTA gets the same number of tiles whatever the lengths are, and the lengths
-// need not be known on the host.  A unit that lies inside one CTA is finished there; of a unit cut by CTA boundaries every CTA
-// leaves (max, sum, unnormalised output), joined in ascending order by the second launch.  The order of every sum depends on
-// the lengths and the number of SMs only: equal calls give equal bits.
+// Split: all (sequence, kv head) units' rows are cut into tiles of 64 (d = 128) or 128 (d = 64) keys, and the list of all tiles into
+// equal ranges, one per CTA; the lengths need not be known on the host.  A unit that lies inside one range is finished there; of a
+// unit cut by range boundaries every CTA leaves (max, sum, unnormalised output), joined in ascending order by the second launch.
+// The ranges depend on the lengths and the number of SMs only: equal calls give equal bits.
+// (SMs do not get quite equal shares of the memory's rate, so ranges of falling sizes, taken as CTAs become free — by the block
+// scheduler, or by clusterlaunchcontrol within running CTAs — were tried; the additional parts cost more than the balance gave:
+// 357 / 358 against 348 us for 4 x 131072 rows of 8 heads, 102 / 106 against 96 us for 64 x 2048 rows on average.)
 #include "catena_math.cuh"
 #include "paged.cuh"
 
@@ -38,12 +40,26 @@ template <int D> struct Shape {
     static constexpr uint32_t kSmem = kRing + kMerge + kWarps * 8 * 2 * 4;
 };
 
-// What a CTA left behind: of the segment that began its unit and did not finish it (slot 1), of the one that continues a unit
-// begun by an earlier CTA (slot 0).  first.x: 1 = slot 1 holds the beginning of a unit; y: unit; z: tiles of the unit in later CTAs
+// The tiles in `ranges` ranges, of which the first `tiles` have one each when there are fewer.
+struct Ranges {
+    uint64_t tiles, n;
+    __device__ __forceinline__ Ranges(uint64_t tiles_, uint32_t ranges) : tiles(tiles_), n(tiles_ < ranges ? tiles_ : ranges) {}
+    __device__ __forceinline__ uint64_t start(uint32_t k) const { return k < n ? k * tiles / n : tiles; }
+    // the range that holds tile t: the greatest k with k tiles / n < t + 1
+    __device__ __forceinline__ uint32_t holder(uint64_t t) const { return (uint32_t)(((t + 1) * n + tiles - 1) / tiles - 1); }
+};
+
+// What the ranges leave behind.  Slot 2 k + 1 holds range k's part of a unit that it began and did not finish, slot 2 k its part of
+// a unit begun by an earlier range.  first[k].x: the last range that holds a part of the unit in slot 2 k + 1 (0: that slot is
+// empty), .y: the unit.  With weights: split[unit] = (k, last) of a unit that is cut, (1, 0) of one that is not.
 struct Partials {
-    uint4* first;       // [C]
-    float2* ml;         // [C][2][16]   (max in base 2, sum)
-    float* o;           // [C][2][hq / hkv][D]
+    uint2* first;       // [ranges]
+    float2* ml;         // [ranges][2][16]   (max in base 2, sum)
+    float* o;           // [ranges][2][hq / hkv][D]
+    uint2* split;       // [units]
+    float2* stats;      // [n_seqs][hq]      (max in base 2, sum) of units that are not cut
+    float* scores;      // [n_seqs][hq][pitch] in base 2
+    uint32_t pitch;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -72,19 +88,15 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
 }
 
-// tiles of one head of all sequences; whole CTA
+// tiles of one head of all sequences; every warp for itself
 template <int TILE>
-__device__ __forceinline__ uint64_t count_tiles(const View& c, uint64_t* sums) {
+__device__ __forceinline__ uint64_t count_tiles(const View& c) {
     uint64_t mine = 0;
-    for (uint32_t b = threadIdx.x; b < c.n_seqs; b += kThreads) mine += (c.length(b) + TILE - 1) / TILE;
+#pragma unroll 4
+    for (uint32_t b = threadIdx.x & 31; b < c.n_seqs; b += 32) mine += (c.length(b) + TILE - 1) / TILE;
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, off);
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    uint64_t all = 0;
-    for (int w = 0; w < kWarps; ++w) all += sums[w];
-    __syncthreads();
-    return all;
+    return mine;
 }
 
 // a position in the list of all tiles: unit (b, h), tile of the unit, rows of the sequence
@@ -106,27 +118,29 @@ struct Cursor {
 
 template <int D, int NT, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel(View c, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ o,
-                                                                                 uint32_t hq, float scale_log2, Partials part,
-                                                                                 float* __restrict__ scores, float2* __restrict__ stats) {
+                                                                                 uint32_t hq, float scale_log2, Partials part) {
     using S = Shape<D>;
     constexpr int KEYS = S::kKeys, TILE = S::kTile, SUB = KEYS / 16, CH = D / 8;     // CH: 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t smem[];
     float* merge = reinterpret_cast<float*>(smem + S::kRing);
     float2* merge_ml = reinterpret_cast<float2*>(smem + S::kRing + S::kMerge);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const uint32_t group = hq / c.hkv, C = gridDim.x, cta = blockIdx.x;
+    const uint32_t group = hq / c.hkv, range = blockIdx.x;
     pdl_trigger();
     pdl_wait();
 
-    for (uint32_t b = cta; b < c.n_seqs; b += C) {                 // a sequence without rows: zeros
-        if (c.length(b) != 0) continue;
-        for (uint32_t i = tid; i < hq * D / 8; i += kThreads) reinterpret_cast<uint4*>(o + (size_t)b * hq * D)[i] = make_uint4(0, 0, 0, 0);
-    }
-    const uint64_t total = count_tiles<TILE>(c, reinterpret_cast<uint64_t*>(merge)) * c.hkv;
-    const uint64_t n_cta = total < C ? total : C;                  // CTAs with work: each has a tile at least
-    const uint64_t t0 = cta < n_cta ? cta * total / n_cta : 0, t1 = cta < n_cta ? (cta + 1) * total / n_cta : 0;
+    const Ranges ranges(count_tiles<TILE>(c) * c.hkv, gridDim.x);
+    const uint64_t t0 = ranges.start(range), t1 = ranges.start(range + 1);
+    // sequences without rows: zeros, written while the first tiles are on their way
+    auto write_zeros = [&] {
+        for (uint32_t b = range; b < c.n_seqs; b += gridDim.x) {
+            if (c.length(b) != 0) continue;
+            for (uint32_t i = tid; i < hq * D / 8; i += kThreads) reinterpret_cast<uint4*>(o + (size_t)b * hq * D)[i] = make_uint4(0, 0, 0, 0);
+        }
+    };
     if (t0 == t1) {
-        if (tid == 0) part.first[cta] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) part.first[range] = make_uint2(0, 0);
+        write_zeros();
         return;
     }
     Cursor<TILE> load;                                             // the tile that is loaded next
@@ -157,8 +171,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
         load.tile = rest - load.h * load.tiles();
     }
     Cursor<TILE> at = load;                                        // the tile that is computed next
-    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStageBytes);
     uint64_t to_load = t1 - t0;
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStageBytes);
 
     // one warp's rows of the tile at `load` into a stage; rows behind the sequence's end are zeros and read nothing
     auto issue = [&](uint32_t stage) {
@@ -187,10 +201,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
     float acc[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int s = 0; s < kStages; ++s) issue(s);
+    write_zeros();
 
-    uint32_t stage = 0;
+    uint32_t stage = 0, seg_first = 0;
     bool fresh = true;                                             // the next tile begins a segment
-    uint32_t seg_first = 0;
     for (uint64_t t = t0; t < t1; ++t) {
         if (fresh) {
             fresh = false;
@@ -242,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
                     if (WEIGHTS) {
                         const uint32_t head = nt * 8 + 2 * t4 + e;
                         if (head < group) {
-                            float* dst = scores + ((size_t)at.b * hq + at.h * group + head) * c.cap();
+                            float* dst = part.scores + ((size_t)at.b * hq + at.h * group + head) * part.pitch;
                             if (live0) dst[key] = s[nt][e];
                             if (live1) dst[key + 8] = s[nt][2 + e];
                         }
@@ -309,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
         // ---- the segment [seg_first, tile] of unit (b, h) is done: join the warps
         fresh = true;
         const bool whole = seg_first == 0 && tile + 1 == unit_tiles;
-        const uint32_t slot = cta * 2 + (seg_first == 0 ? 1u : 0u);
+        const uint32_t slot = range * 2 + (seg_first == 0 ? 1u : 0u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -342,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
                 const size_t out_head = (size_t)b * hq + h * group + head;
                 if (whole) {
                     o[out_head * D + d] = __float2bfloat16_rn(L == 0.0f ? 0.0f : __fdiv_rn(O, L));
-                    if (WEIGHTS && d == 0) stats[out_head] = make_float2(M, L);
+                    if (WEIGHTS && d == 0) part.stats[out_head] = make_float2(M, L);
                 } else {
                     part.o[((size_t)slot * group + head) * D + d] = O;
                     if (d == 0) part.ml[slot * 16 + head] = make_float2(M, L);
@@ -350,88 +364,159 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_paged_kernel
             }
             __syncthreads();
         }
-        if (t + 1 == t1 && tid == 0)
-            part.first[cta] = !whole && seg_first == 0 ? make_uint4(1, b * c.hkv + h, unit_tiles - (tile + 1), 0) : make_uint4(0, 0, 0, 0);
+        if (tid == 0) {
+            const bool begun = !whole && seg_first == 0;               // then this is the range's last tile
+            uint2 f = make_uint2(0, 0);
+            if (begun) f = make_uint2(ranges.holder(t + (unit_tiles - tile - 1)), b * c.hkv + h);
+            if (t + 1 == t1) part.first[range] = f;
+            if (WEIGHTS && seg_first == 0) part.split[b * c.hkv + h] = begun ? make_uint2(range, f.x) : make_uint2(1, 0);
+        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Joins the parts of a unit that was cut: CTA c does it for the unit that CTA c of the first launch began and did not finish.
-// `tiles_left` tiles of it lie in the CTAs behind, which hold the same numbers of tiles the first launch computed.
-template <int D>
-__global__ void __launch_bounds__(kThreads) attn_decode_paged_join_kernel(View c, __nv_bfloat16* __restrict__ o, uint32_t hq, Partials part,
-                                                                          float2* __restrict__ stats) {
-    __shared__ uint64_t sums[kWarps];
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t cta = blockIdx.x, C = gridDim.x, tid = threadIdx.x, group = hq / c.hkv;
-    const uint4 f = part.first[cta];
-    if (f.x == 0) return;
-    const uint64_t total = count_tiles<Shape<D>::kTile>(c, sums) * c.hkv;
-    const uint64_t n_cta = total < C ? total : C;
-    const uint64_t stop = (cta + 1) * total / n_cta + f.z;               // first tile behind the unit
-    const uint32_t last = (uint32_t)((stop * n_cta + total - 1) / total - 1);     // the CTA that holds tile stop - 1
-    const uint32_t b = f.y / c.hkv, h = f.y % c.hkv;
-    for (uint32_t i = tid; i < group * D; i += kThreads) {
-        const uint32_t head = i / D, d = i % D;
-        float M = part.ml[(cta * 2 + 1) * 16 + head].x;
-        for (uint32_t s = cta + 1; s <= last; ++s) M = fmaxf(M, part.ml[s * 2 * 16 + head].x);
-        float L = 0.0f, O = 0.0f;
-        for (uint32_t s = cta; s <= last; ++s) {
-            const uint32_t slot = s * 2 + (s == cta ? 1u : 0u);
-            const float2 ml = part.ml[slot * 16 + head];
-            const float w = ml.x == M ? 1.0f : ex2(__fsub_rn(ml.x, M));
-            L = __fmaf_rn(ml.y, w, L);
-            O = __fmaf_rn(part.o[((size_t)slot * group + head) * D + d], w, O);
-        }
-        const size_t out_head = (size_t)b * hq + h * group + head;
-        o[out_head * D + d] = __float2bfloat16_rn(L == 0.0f ? 0.0f : __fdiv_rn(O, L));
-        if (stats && d == 0) stats[out_head] = make_float2(M, L);
-    }
-}
+// CTAs below `ranges` join the parts of a unit that was cut: CTA k does it for the unit that range k began and did not finish.
+// The other CTAs (only with weights) do weights_out[j] = weights_in[j] + sum over the group's heads, ascending, of exp2(s_j - M) / L
+// for kWeightRows rows of a unit; they join (M, L) of a cut unit for themselves.
+constexpr int kJoinThreads = 256;
+constexpr int kWeightRows = kJoinThreads * 4;
 
-// weights_out[j] = weights_in[j] + sum over the group's heads, in ascending order, of exp2(s_j - M) / L
-__global__ void __launch_bounds__(256) attn_decode_paged_weights_kernel(View c, uint32_t hq, const float* __restrict__ scores, const float2* __restrict__ stats,
-                                                                        const float* weights_in, float* weights_out) {
-    __shared__ float s_m[16], s_r[16];
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t unit = blockIdx.y, b = unit / c.hkv, group = hq / c.hkv, tid = threadIdx.x;
-    const uint32_t n = c.length(b), j0 = blockIdx.x * 1024;
-    if (j0 >= n) return;
-    if (tid < group) {
-        const float2 ml = stats[(size_t)unit * group + tid];
-        s_m[tid] = ml.x == -INFINITY ? 0.0f : ml.x;
-        s_r[tid] = ml.y == 0.0f ? 0.0f : __frcp_rn(ml.y);
+// M and L of the group's heads over slots k (+ 1 of the first) .. last, to s_m and s_l; whole CTA
+__device__ __forceinline__ void join_stats(const Partials& part, uint32_t k, uint32_t last, uint32_t group, float (*s_part)[16], float* s_m, float* s_l) {
+    const uint32_t head = threadIdx.x & 15, lane16 = threadIdx.x >> 4;           // 16 threads per head
+    float m = -INFINITY;
+    if (head < group)
+        for (uint32_t s = k + lane16; s <= last; s += kJoinThreads / 16) m = fmaxf(m, part.ml[(s * 2 + (s == k)) * 16 + head].x);
+    s_part[lane16][head] = m;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        for (int i = 1; i < kJoinThreads / 16; ++i) m = fmaxf(m, s_part[i][head]);
+        s_m[head] = m;
     }
     __syncthreads();
-    for (uint32_t j = j0 + tid; j < min(j0 + 1024, n); j += 256) {
-        float w = 0.0f;
-        for (uint32_t i = 0; i < group; ++i) w = __fmaf_rn(ex2(__fsub_rn(scores[((size_t)unit * group + i) * c.cap() + j], s_m[i])), s_r[i], w);
-        const size_t at = (size_t)unit * c.cap() + j;
-        weights_out[at] = weights_in ? __fadd_rn(weights_in[at], w) : w;
+    m = s_m[head];
+    float l = 0.0f;
+    if (head < group)
+        for (uint32_t s = k + lane16; s <= last; s += kJoinThreads / 16) {
+            const float2 ml = part.ml[(s * 2 + (s == k)) * 16 + head];
+            l = __fmaf_rn(ml.y, ml.x == m ? 1.0f : ex2(__fsub_rn(ml.x, m)), l);
+        }
+    s_part[lane16][head] = l;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        for (int i = 1; i < kJoinThreads / 16; ++i) l = __fadd_rn(l, s_part[i][head]);
+        s_l[head] = l;
     }
+    __syncthreads();
+}
+
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(View c, __nv_bfloat16* __restrict__ o, uint32_t hq, uint32_t ranges, Partials part,
+                                                                              const float* weights_in, float* weights_out) {
+    __shared__ float s_part[kJoinThreads / 16][16], s_m[16], s_l[16];
+    __shared__ float4 s_o[kJoinThreads];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tid = threadIdx.x, group = hq / c.hkv;
+    if (blockIdx.x < ranges) {
+        const uint32_t k = blockIdx.x;
+        const uint2 f = part.first[k];
+        if (f.x == 0) return;
+        const uint32_t last = f.x, b = f.y / c.hkv, h = f.y % c.hkv;
+        join_stats(part, k, last, group, s_part, s_m, s_l);
+        // a thread has four elements of a head; where the group has few heads, several threads share the parts of one
+        const uint32_t items = group * (D / 4), team = items < kJoinThreads ? kJoinThreads / items : 1;
+        for (uint32_t i0 = 0; i0 < items; i0 += kJoinThreads) {
+            const uint32_t item = i0 + tid % min(items, (uint32_t)kJoinThreads), member = tid / min(items, (uint32_t)kJoinThreads);
+            const uint32_t head = item / (D / 4), d4 = item % (D / 4);
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (member < team && item < items) {
+                const float M = s_m[head];
+#pragma unroll 4
+                for (uint32_t s = k + member; s <= last; s += team) {
+                    const uint32_t slot = s * 2 + (s == k);
+                    const float m = part.ml[slot * 16 + head].x, w = m == M ? 1.0f : ex2(__fsub_rn(m, M));
+                    const float4 v = reinterpret_cast<const float4*>(part.o)[(slot * group + head) * (D / 4) + d4];
+                    sum.x = __fmaf_rn(v.x, w, sum.x);
+                    sum.y = __fmaf_rn(v.y, w, sum.y);
+                    sum.z = __fmaf_rn(v.z, w, sum.z);
+                    sum.w = __fmaf_rn(v.w, w, sum.w);
+                }
+            }
+            __syncthreads();
+            s_o[tid] = sum;
+            __syncthreads();
+            if (member == 0 && item < items) {
+                for (uint32_t j = 1; j < team; ++j) {
+                    const float4 v = s_o[j * items + tid];
+                    sum.x = __fadd_rn(sum.x, v.x);
+                    sum.y = __fadd_rn(sum.y, v.y);
+                    sum.z = __fadd_rn(sum.z, v.z);
+                    sum.w = __fadd_rn(sum.w, v.w);
+                }
+                const float L = s_l[head], r = L == 0.0f ? 0.0f : __frcp_rn(L);
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(L == 0.0f ? 0.0f : __fmul_rn(sum.x, r), L == 0.0f ? 0.0f : __fmul_rn(sum.y, r));
+                const __nv_bfloat162 hi = __floats2bfloat162_rn(L == 0.0f ? 0.0f : __fmul_rn(sum.z, r), L == 0.0f ? 0.0f : __fmul_rn(sum.w, r));
+                const size_t at = ((size_t)b * hq + h * group + head) * D + d4 * 4;
+                *reinterpret_cast<uint2*>(o + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+        }
+        return;
+    }
+    const uint32_t blocks = (c.cap() + kWeightRows - 1) / kWeightRows, at = blockIdx.x - ranges;
+    const uint32_t unit = at / blocks, j0 = at % blocks * kWeightRows, b = unit / c.hkv;
+    const uint32_t n = c.length(b);
+    if (j0 >= n) return;
+    const uint2 cut = part.split[unit];
+    if (cut.x <= cut.y) {
+        join_stats(part, cut.x, cut.y, group, s_part, s_m, s_l);
+    } else if (tid < group) {
+        const float2 ml = part.stats[(size_t)unit * group + tid];
+        s_m[tid] = ml.x;
+        s_l[tid] = ml.y;
+    }
+    __syncthreads();
+    const uint32_t j = j0 + tid * 4;
+    if (j >= n) return;
+    float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float* sc = part.scores + (size_t)unit * group * part.pitch + j;       // the pitch is a multiple of 4
+#pragma unroll 4
+    for (uint32_t i = 0; i < group; ++i) {
+        const float4 s = *reinterpret_cast<const float4*>(sc + (size_t)i * part.pitch);
+        const float m = s_m[i] == -INFINITY ? 0.0f : s_m[i], r = s_l[i] == 0.0f ? 0.0f : __frcp_rn(s_l[i]);
+        w.x = __fmaf_rn(ex2(__fsub_rn(s.x, m)), r, w.x);
+        w.y = __fmaf_rn(ex2(__fsub_rn(s.y, m)), r, w.y);
+        w.z = __fmaf_rn(ex2(__fsub_rn(s.z, m)), r, w.z);
+        w.w = __fmaf_rn(ex2(__fsub_rn(s.w, m)), r, w.w);
+    }
+    const float ws[4] = {w.x, w.y, w.z, w.w};
+    const size_t to = (size_t)unit * c.cap() + j;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+        if (j + e < n) weights_out[to + e] = weights_in ? __fadd_rn(weights_in[to + e], ws[e]) : ws[e];
 }
 
 // ---------------------------------------------------------------- host side
 struct Plan {
-    uint32_t ctas;
-    uint64_t first, ml, o, stats, scores, bytes;       // byte offsets into the workspace
+    uint32_t ranges, pitch;
+    uint64_t first, ml, o, split, stats, scores, bytes;       // byte offsets into the workspace
 };
 static Plan plan_for(const View& c, uint64_t d, uint64_t hq, bool weights) {
     Plan p = {};
-    int sms = tls().sm_count > 0 ? tls().sm_count : 148;
+    const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148;
     const uint64_t tile = d == 128 ? Shape<128>::kTile : Shape<64>::kTile;
     const uint64_t most = (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), tile);      // tiles when every sequence is full
-    p.ctas = (uint32_t)(most < (uint64_t)sms * kCtasPerSm ? most : (uint64_t)sms * kCtasPerSm);
-    const uint64_t group = hq / c.hkv;
+    p.ranges = (uint32_t)(most < sms * kCtasPerSm ? most : sms * kCtasPerSm);
+    const uint64_t group = hq / c.hkv, ranges = p.ranges, units = (uint64_t)c.n_seqs * c.hkv;
     auto take = [&](uint64_t bytes) { const uint64_t at = p.bytes; p.bytes += (bytes + 255) & ~255ull; return at; };
-    p.first = take(p.ctas * sizeof(uint4));
-    p.ml = take((uint64_t)p.ctas * 2 * 16 * sizeof(float2));
-    p.o = take((uint64_t)p.ctas * 2 * group * d * sizeof(float));
+    p.first = take(ranges * sizeof(uint2));
+    p.ml = take(ranges * 2 * 16 * sizeof(float2));
+    p.o = take(ranges * 2 * group * d * sizeof(float));
     if (weights) {
+        p.pitch = (c.cap() + 3) & ~3u;
+        p.split = take(units * sizeof(uint2));
         p.stats = take((uint64_t)c.n_seqs * hq * sizeof(float2));
-        p.scores = take((uint64_t)c.n_seqs * hq * c.cap() * sizeof(float));
+        p.scores = take((uint64_t)c.n_seqs * hq * p.pitch * sizeof(float));
     }
     return p;
 }
@@ -441,15 +526,22 @@ static catena_status_t check_heads(const View& c, uint64_t hq) {
 }
 
 template <int D, int NT, bool WEIGHTS>
-static catena_status_t launch_attention(const View& c, const Plan& p, const void* q, void* o, uint64_t hq, float scale, uint8_t* ws) {
+static catena_status_t launch_attention(const View& c, const Plan& p, const void* q, void* o, uint64_t hq, float scale, const float* weights_in,
+                                        float* weights_out, uint8_t* ws) {
     auto kernel = attn_decode_paged_kernel<D, NT, WEIGHTS>;
     CATENA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem));
-    const Partials part = {(uint4*)(ws + p.first), (float2*)(ws + p.ml), (float*)(ws + p.o)};
-    float2* stats = WEIGHTS ? (float2*)(ws + p.stats) : nullptr;
-    CATENA_TRY(launch("attn_decode_paged_kernel", kernel, dim3(p.ctas), dim3(kThreads), Shape<D>::kSmem, c, (const __nv_bfloat16*)q,
-                      (__nv_bfloat16*)o, (uint32_t)hq, scale * 1.44269504088896340736f, part, WEIGHTS ? (float*)(ws + p.scores) : nullptr, stats));
-    return launch("attn_decode_paged_join_kernel", attn_decode_paged_join_kernel<D>, dim3(p.ctas), dim3(kThreads), 0, c, (__nv_bfloat16*)o,
-                  (uint32_t)hq, part, stats);
+    Partials part = {(uint2*)(ws + p.first), (float2*)(ws + p.ml), (float*)(ws + p.o), nullptr, nullptr, nullptr, p.pitch};
+    uint64_t ctas = p.ranges;
+    if (WEIGHTS) {
+        part.split = (uint2*)(ws + p.split);
+        part.stats = (float2*)(ws + p.stats);
+        part.scores = (float*)(ws + p.scores);
+    }
+    CATENA_TRY(launch("attn_decode_paged_kernel", kernel, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, c, (const __nv_bfloat16*)q,
+                      (__nv_bfloat16*)o, (uint32_t)hq, scale * 1.44269504088896340736f, part));
+    if (WEIGHTS) ctas += (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), kWeightRows);
+    return launch("attn_decode_paged_join_kernel", attn_decode_paged_join_kernel<D>, dim3((unsigned)ctas), dim3(kJoinThreads), 0, c, (__nv_bfloat16*)o,
+                  (uint32_t)hq, p.ranges, part, weights_in, weights_out);
 }
 
 }  // namespace paged
@@ -474,21 +566,17 @@ catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache
     if (!aligned16(q) || !aligned16(o) || !aligned4(weights_in) || !aligned4(weights_out) || ((uintptr_t)workspace & 255))
         return fail(CATENA_E_BAD_ARG, "attn_decode_paged: q and o must be 16-byte aligned, the workspace 256-byte");
     if (scale - scale != 0.0f) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite");
-    if (weights_out && (uint64_t)c.n_seqs * c.hkv > 65535) return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: weights of more than 65535 (sequence, kv head) pairs");
+    if ((uint64_t)c.n_seqs * c.hkv > 0x7FFFFFFFull || (weights_out && (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), kWeightRows) > 0x7FFF0000ull))
+        return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: more (sequence, kv head) pairs than the kernels index");
     CATENA_TRY(begin(&c.err));
     const Plan p = plan_for(c, cache->head_dim, n_heads, weights_out != nullptr);
     if (workspace_bytes < p.bytes) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: workspace too small");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool wide = n_heads / c.hkv > 8, w = weights_out != nullptr;
-    using Fn = catena_status_t (*)(const View&, const Plan&, const void*, void*, uint64_t, float, uint8_t*);
+    using Fn = catena_status_t (*)(const View&, const Plan&, const void*, void*, uint64_t, float, const float*, float*, uint8_t*);
     static const Fn table[2][2][2] = {{{launch_attention<64, 1, false>, launch_attention<64, 1, true>}, {launch_attention<64, 2, false>, launch_attention<64, 2, true>}},
                                       {{launch_attention<128, 1, false>, launch_attention<128, 1, true>}, {launch_attention<128, 2, false>, launch_attention<128, 2, true>}}};
-    CATENA_TRY(table[cache->head_dim == 128][wide][w](c, p, q, o, n_heads, scale, ws));
-    if (w) {
-        const dim3 grid((unsigned)ceil_div_u64(c.cap(), 1024), c.n_seqs * c.hkv);
-        CATENA_TRY(launch("attn_decode_paged_weights_kernel", attn_decode_paged_weights_kernel, grid, dim3(256), 0, c, (uint32_t)n_heads,
-                          (const float*)(ws + p.scores), (const float2*)(ws + p.stats), weights_in, weights_out));
-    }
+    CATENA_TRY(table[cache->head_dim == 128][wide][w](c, p, q, o, n_heads, scale, weights_in, weights_out, ws));
     return end();
 }
 
