@@ -62,21 +62,29 @@ static inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+struct How {
+    uint32_t cluster = 1;
+    bool early = true;      // may start while the launch before it still runs
+};
 template <class... KArgs, class... Args>
-static catena_status_t launch_cluster(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, uint32_t cluster, Args... args) {
+static catena_status_t launch_as(How how, const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = tls().stream;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cluster;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    if (how.early) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (how.cluster > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = how.cluster;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
     if (e != cudaSuccess) return fail_cuda(e, what);
     count_launch();
@@ -84,7 +92,7 @@ static catena_status_t launch_cluster(const char* what, void (*kernel)(KArgs...)
 }
 template <class... KArgs, class... Args>
 static catena_status_t launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
-    return launch_cluster(what, kernel, grid, block, smem, 1, args...);
+    return launch_as(How(), what, kernel, grid, block, smem, args...);
 }
 #endif
 

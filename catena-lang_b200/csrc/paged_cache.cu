@@ -551,7 +551,7 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     if (units > 65535) return fail(CATENA_E_TOO_LARGE, "kv_evict_paged: more than 65535 (sequence, kv head) pairs");
     CATENA_TRY(begin(&c.err));
     // A CTA per 1024 rows that a sequence may have, up to eight and as long as every CTA has an SM of its own.  (Clusters of small
-    // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take SELTIME.)  The shared memory that keeps a second CTA
+    // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take 17.)  The shared memory that keeps a second CTA
     // off the SM is asked for whether it is filled or not.
     const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148;
     uint32_t ctas = 1;
@@ -561,7 +561,9 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     size_t smem = (size_t)room * 4 + room / 8;
     if (ctas > 1 && smem < kSelAlone) smem = kSelAlone;
     if (smem > 32768) CATENA_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelRoom * 4 + kSelRoom / 8));
-    CATENA_TRY(launch_cluster("evict_select_kernel", evict_select_kernel, dim3((unsigned)units * ctas), dim3(kSelThreads), smem, ctas, c, weights,
+    How how;
+    how.cluster = ctas;
+    CATENA_TRY(launch_as(how, "evict_select_kernel", evict_select_kernel, dim3((unsigned)units * ctas), dim3(kSelThreads), smem, c, weights,
                               (uint32_t)budget, (uint32_t)recent, lengths_out, weights_out, (uint32_t)(max_pages_out * c.page_size), kept,
                               (int32_t*)workspace, room));
     const uint64_t rows_per_cta = 4 * (256 / (cache->head_dim / 8));
