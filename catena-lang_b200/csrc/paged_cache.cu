@@ -94,7 +94,11 @@ __global__ void rope_angles_kernel(InvFreq inv, float2* __restrict__ out, uint32
 // Token t of sequence b (token_start[b] <= t < token_start[b + 1]) is the (t - token_start[b])-th of the sequence's new rows, which
 // are its last: row = length - new + nth, position = positions[b] + nth.  Rotation (rotate half, products and sum rounded
 // separately as in llama.cu): (x1 c - x2 s, x2 c + x1 s).
-// One thread per (token, head, 8 pairs).  The sequence of a token is found by a whole warp at once, 32 boundaries per step.
+// A CTA has a token: a thread 8 pairs of every 16th (d = 128) or 32nd head, so the angles and the row's place are found once for all
+// of them, and three heads' loads are on their way at once.  Few tokens: the heads over several CTAs.  The sequence of a token is found
+// by a whole warp at once, 32 boundaries per step.
+// Bound: HBM, every element is read and written once (9219 tokens of 16 + 32 heads of 128: 38.7 us,
+// 5.3 TB/s; with a thread per head and pair group, which looks everything up for itself, 45 us).
 __device__ __forceinline__ uint32_t find_seq(const int32_t* __restrict__ start, uint32_t n, int64_t t) {
     // the largest b with start[b] <= t, for start[0] <= t; whole warp
     uint32_t lo = 0, width = n + 1;                    // boundaries lo .. lo + width - 1 can still be it
@@ -114,9 +118,11 @@ __device__ __forceinline__ uint32_t find_seq(const int32_t* __restrict__ start, 
 template <int D>
 __global__ void __launch_bounds__(128) rope_append_paged_kernel(View c, const __nv_bfloat16* __restrict__ qkv, uint64_t pitch,
                                                                 const int32_t* __restrict__ token_start, const int32_t* __restrict__ positions,
-                                                                const float2* __restrict__ angles, uint32_t n_angles, uint32_t hq,
+                                                                const float4* __restrict__ angles, uint32_t n_angles, uint32_t hq,
                                                                 __nv_bfloat16* __restrict__ q_out) {
     constexpr uint32_t kPieces = D / 16;               // 8 pairs each
+    constexpr uint32_t kHeads = 128 / kPieces;
+    constexpr int kAtOnce = 3;
     pdl_trigger();
     pdl_wait();
     const uint32_t t = blockIdx.x;
@@ -128,60 +134,71 @@ __global__ void __launch_bounds__(128) rope_append_paged_kernel(View c, const __
         nth = t - (uint32_t)token_start[b];
         fresh = (uint32_t)(token_start[b + 1] - token_start[b]);
     }
-    const uint32_t idx = blockIdx.y * 128 + threadIdx.x, head = idx / kPieces, i0 = idx % kPieces * 8;
-    const uint32_t heads = hq + 2 * c.hkv;
-    if (head >= heads) return;
     const uint32_t n = c.length(b);
     if (fresh > n) {
         atomicOr(c.err, kErrLength);
         return;
     }
-    uint32_t dst_row = 0;
-    if (head >= hq) {
-        dst_row = c.row(b, (head - hq) % c.hkv, n - fresh + nth);
-        if (dst_row == kNoRow) return;
+    const uint32_t r = n - fresh + nth, i0 = threadIdx.x % kPieces * 8;
+    const int64_t pos = (positions ? (int64_t)positions[b] : (int64_t)(n - fresh)) + nth;
+    const uint32_t row0 = c.row(b, 0, r);              // that of kv head 0; a head's are page_size rows on
+    if (pos < 0 || pos >= (int64_t)n_angles) {
+        atomicOr(c.err, kErrPosition);
+        return;
     }
-    const __nv_bfloat16* src = qkv + (size_t)t * pitch + head * D;
-    const uint4 lo = *reinterpret_cast<const uint4*>(src + i0), hi = *reinterpret_cast<const uint4*>(src + D / 2 + i0);
-    __nv_bfloat16* dst;
-    uint4 out_lo = lo, out_hi = hi;
-    if (head >= hq + c.hkv) {
-        dst = c.v + (size_t)dst_row * D;
-    } else {
-        const int64_t pos = (positions ? (int64_t)positions[b] : (int64_t)(n - fresh)) + nth;
-        if (pos < 0 || pos >= (int64_t)n_angles) {
-            atomicOr(c.err, kErrPosition);
-            return;
-        }
-        const float4* cs = reinterpret_cast<const float4*>(angles + (size_t)pos * (D / 2) + i0);
-        const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
-        uint32_t r1[4], r2[4];
+    float4 cs[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float4 a = cs[e];
-            const float x10 = __uint_as_float(lw[e] << 16), x11 = __uint_as_float(lw[e] & 0xFFFF0000u);
-            const float x20 = __uint_as_float(hw[e] << 16), x21 = __uint_as_float(hw[e] & 0xFFFF0000u);
-            const __nv_bfloat162 o1 = __floats2bfloat162_rn(cmath::sub(cmath::mul(x10, a.x), cmath::mul(x20, a.y)),
-                                                            cmath::sub(cmath::mul(x11, a.z), cmath::mul(x21, a.w)));
-            const __nv_bfloat162 o2 = __floats2bfloat162_rn(cmath::add(cmath::mul(x20, a.x), cmath::mul(x10, a.y)),
-                                                            cmath::add(cmath::mul(x21, a.z), cmath::mul(x11, a.w)));
-            r1[e] = *reinterpret_cast<const uint32_t*>(&o1);
-            r2[e] = *reinterpret_cast<const uint32_t*>(&o2);
+    for (int e = 0; e < 4; ++e) cs[e] = angles[((size_t)pos * (D / 2) + i0) / 2 + e];
+    const uint32_t heads = hq + 2 * c.hkv, step = kHeads * gridDim.y;
+    for (uint32_t h0 = blockIdx.y * kHeads + threadIdx.x / kPieces; h0 < heads; h0 += kAtOnce * step) {
+        uint4 lo[kAtOnce], hi[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const uint32_t head = h0 + u * step;
+            if (head >= heads) break;
+            const __nv_bfloat16* src = qkv + (size_t)t * pitch + head * D + i0;
+            lo[u] = *reinterpret_cast<const uint4*>(src);
+            hi[u] = *reinterpret_cast<const uint4*>(src + D / 2);
         }
-        out_lo = make_uint4(r1[0], r1[1], r1[2], r1[3]);
-        out_hi = make_uint4(r2[0], r2[1], r2[2], r2[3]);
-        dst = head < hq ? q_out + ((size_t)t * hq + head) * D : c.k + (size_t)dst_row * D;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const uint32_t head = h0 + u * step;
+            if (head >= heads) break;
+            if (head >= hq && row0 == kNoRow) continue;
+            __nv_bfloat16* dst;
+            if (head < hq) dst = q_out + ((size_t)t * hq + head) * D;
+            else if (head < hq + c.hkv) dst = c.k + (size_t)(row0 + (head - hq) * c.page_size) * D;
+            else dst = c.v + (size_t)(row0 + (head - hq - c.hkv) * c.page_size) * D;
+            if (head < hq + c.hkv) {
+                const uint32_t lw[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, hw[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+                uint32_t r1[4], r2[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 a = cs[e];
+                    const float x10 = __uint_as_float(lw[e] << 16), x11 = __uint_as_float(lw[e] & 0xFFFF0000u);
+                    const float x20 = __uint_as_float(hw[e] << 16), x21 = __uint_as_float(hw[e] & 0xFFFF0000u);
+                    const __nv_bfloat162 o1 = __floats2bfloat162_rn(cmath::sub(cmath::mul(x10, a.x), cmath::mul(x20, a.y)),
+                                                                    cmath::sub(cmath::mul(x11, a.z), cmath::mul(x21, a.w)));
+                    const __nv_bfloat162 o2 = __floats2bfloat162_rn(cmath::add(cmath::mul(x20, a.x), cmath::mul(x10, a.y)),
+                                                                    cmath::add(cmath::mul(x21, a.z), cmath::mul(x11, a.w)));
+                    r1[e] = *reinterpret_cast<const uint32_t*>(&o1);
+                    r2[e] = *reinterpret_cast<const uint32_t*>(&o2);
+                }
+                lo[u] = make_uint4(r1[0], r1[1], r1[2], r1[3]);
+                hi[u] = make_uint4(r2[0], r2[1], r2[2], r2[3]);
+            }
+            *reinterpret_cast<uint4*>(dst + i0) = lo[u];
+            *reinterpret_cast<uint4*>(dst + D / 2 + i0) = hi[u];
+        }
     }
-    *reinterpret_cast<uint4*>(dst + i0) = out_lo;
-    *reinterpret_cast<uint4*>(dst + D / 2 + i0) = out_hi;
 }
 
 // ---------------------------------------------------------------- eviction: which rows stay
-// A cluster of CTAs per (sequence, kv head), each with a stretch of the rows, whose weights it keeps in shared memory as
-// order-preserving bits.  Rows 0 .. n - recent - 1 compete by weight for budget - recent places; the limit is found by a radix
-// select, 2048 bins between the least and the greatest weight (weights spread over few octaves, so bins cut from the top bits
-// would hold thousands each, and the updates of their counters queue up), every CTA adding up all CTAs' bins for itself.  One pass
-// usually leaves a bin of at most 256 rows, which are ranked by comparing them with each other; ties at the limit go to the lowest rows.
+// A cluster of CTAs per (sequence, kv head), each with a stretch of the rows, whose weights it keeps in shared memory.  Rows
+// 0 .. n - recent - 1 compete by weight for budget - recent places; the limit is found by a radix select over the weights'
+// order-preserving bits, 2048 bins between the least and the greatest of a sample, which every CTA takes alike (weights spread over
+// few octaves: bins cut from the top bits would hold thousands each), every CTA adding up all CTAs' bins for itself.  One pass usually
+// leaves a bin of at most 256 rows, which are ranked by comparing them with each other; ties at the limit go to the lowest rows.
 // A NaN counts as -inf and -0 as +0, so the order is total.  What stays is then written in order: every warp counts in its part
 // of the stretch and writes once it knows how many stay before it.
 constexpr int kSelThreads = 512;
@@ -218,13 +235,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
                                                                    int32_t* __restrict__ lengths_out, float* __restrict__ weights_out,
                                                                    uint32_t cap_out, int32_t* __restrict__ kept, int32_t* __restrict__ rows_ws,
                                                                    uint32_t room) {
-    extern __shared__ uint32_t sel_smem[];             // [room] bits of the stretch's weights, [room / 32] who stays
+    extern __shared__ uint32_t sel_smem[];             // [room] the stretch's weights, [room / 32] who stays
     __shared__ __align__(8) uint32_t hist[kBins];
     __shared__ uint64_t cand[kRanked], all[kRanked];
     __shared__ uint32_t warp_sums[32], s_lo, s_hi, s_digit, s_left, s_count, s_n, s_equal, s_stay;
     __shared__ uint64_t s_limit;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();                                     // only now: the copies below begin before this kernel is done
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t unit = blockIdx.x / ctas, b = unit / c.hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -247,43 +264,43 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
     const uint32_t m = n - recent, want = budget - recent;         // want < m
     const uint32_t part = (n + ctas * kSelWarps * 32 - 1) / (ctas * kSelWarps * 32) * 32;      // rows of a warp
     const uint32_t r0 = min(n, rank * kSelWarps * part), r1 = min(n, r0 + kSelWarps * part), c1 = min(r1, max(m, r0));
-    uint32_t* bits = sel_smem;
+    float* own = reinterpret_cast<float*>(sel_smem);
     uint32_t* words = sel_smem + room;
     const bool held = kSelWarps * part <= room;                    // else the weights are read again in every pass
-    auto key = [&](uint32_t i) { return held ? bits[i - r0] : order_bits(w[i]); };
+    auto weight = [&](uint32_t i) { return held ? own[i - r0] : w[i]; };
+    auto key = [&](uint32_t i) { return order_bits(weight(i)); };
     // a value of every CTA of the cluster, lane q that of CTA q (0 behind the last)
     auto of_all = [&](uint32_t* mine) { return lane < ctas ? *cluster.map_shared_rank(mine, lane) : 0u; };
 
     if (tid == 0) { s_lo = 0xFFFFFFFFu; s_hi = 0; s_n = s_equal = 0; }
     for (uint32_t i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    const uint32_t sample = order_bits(w[(uint32_t)((uint64_t)tid * m / kSelThreads)]);
+    if (held) {
+#pragma unroll 4
+        for (uint32_t i = r0 + tid; i < r1; i += kSelThreads) own[i - r0] = w[i];
+    }
     __syncthreads();
     {
-        uint32_t lo = 0xFFFFFFFFu, hi = 0;
-#pragma unroll 4
-        for (uint32_t i = r0 + tid; i < r1; i += kSelThreads) {
-            const uint32_t u = order_bits(w[i]);
-            if (held) bits[i - r0] = u;
-            if (i < m) { lo = min(lo, u); hi = max(hi, u); }
-        }
-        lo = __reduce_min_sync(0xFFFFFFFFu, lo);
-        hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+        const uint32_t lo = __reduce_min_sync(0xFFFFFFFFu, sample), hi = __reduce_max_sync(0xFFFFFFFFu, sample);
         if (lane == 0) {
             atomicMin(&s_lo, lo);
             atomicMax(&s_hi, hi);
         }
     }
+    __syncthreads();
     uint64_t limit = ~0ull;                                        // a row stays when (bits, lowest row first) reaches it
     if (want) {
-        cluster.sync();
-        const uint32_t his = of_all(&s_hi), los = lane < ctas ? *cluster.map_shared_rank(&s_lo, lane) : 0xFFFFFFFFu;
-        uint32_t lo = __reduce_min_sync(0xFFFFFFFFu, los);
-        uint32_t span = __reduce_max_sync(0xFFFFFFFFu, his) - lo, left = want, count;      // keys lo .. lo + span; the left-th greatest
+        // Keys from lo on in bins of 2^shift, the last bin open above; in the first pass those below lo are in the first bin, and
+        // afterwards all that can hold the limit, the left-th greatest of them, are lo .. lo + span.
+        uint32_t lo = s_lo, span = s_hi - lo, left = want, count;
         int shift = max(0, 21 - __clz(span));                      // span >> shift < 2048 (clz(0) is 32)
+        bool first = true;
         while (true) {
 #pragma unroll 4
             for (uint32_t i = r0 + tid; i < c1; i += kSelThreads) {
-                const uint32_t d = key(i) - lo;
-                if (d <= span) atomicAdd(&hist[d >> shift], 1u);
+                const uint32_t u = key(i);
+                if (first) atomicAdd(&hist[u < lo ? 0u : min((u - lo) >> shift, kBins - 1)], 1u);
+                else if (u - lo <= span) atomicAdd(&hist[(u - lo) >> shift], 1u);
             }
             cluster.sync();
             // the bin of the left-th greatest: sums from the top
@@ -309,12 +326,22 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
                 above += h[e];
             }
             __syncthreads();
+            const uint32_t base = lo, end = lo + span;
             lo += s_digit << shift;
             span = (1u << shift) - 1;
+            if (first && s_digit == 0) {
+                span += base;
+                lo = 0;
+            } else if (first && s_digit == kBins - 1) {
+                span = ~0u - lo;
+            } else if (!first) {
+                span = min(span, end - lo);                        // the last bin may reach past what is left
+            }
+            first = false;
             left = s_left;
             count = s_count;
-            if (count <= kRanked || shift == 0) break;
-            shift = max(0, shift - 11);
+            if (count <= kRanked || span == 0) break;
+            shift = max(0, 21 - __clz(span));
             cluster.sync();                                        // everyone has read the bins
             for (uint32_t i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
@@ -365,7 +392,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
         __syncthreads();
         limit = s_limit;
     }
-    __syncthreads();                                               // `bits` is complete, warp_sums of the tie search has been read
+    __syncthreads();                                               // warp_sums of the tie search has been read
     auto stays = [&](uint32_t i) { return i < r1 && (i >= m || ((uint64_t)key(i) << 32 | (uint32_t)~i) >= limit); };
     const uint32_t i0 = r0 + warp * part;
     uint32_t mine = 0;
@@ -390,28 +417,34 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
             const uint32_t to = at + __popc(votes & ((1u << lane) - 1));
             rows[to] = (int32_t)(i + lane);
             if (kept_row) kept_row[to] = (int32_t)(i + lane);
-            w_out[to] = w[i + lane];
+            w_out[to] = weight(i + lane);
         }
         at += __popc(votes);
     }
 }
 
 // ---------------------------------------------------------------- eviction: the rows that stay, into their new pages
+// The recent rows stay whatever the weights are, and all rows of a sequence within its budget: CTAs that have only such rows copy
+// while the selection still runs (which starts them only once everything before it is done).
 template <int D>
-__global__ void __launch_bounds__(256) evict_copy_kernel(View c, const int32_t* __restrict__ rows_ws, uint32_t budget,
+__global__ void __launch_bounds__(256) evict_copy_kernel(View c, const int32_t* rows_ws, uint32_t budget, uint32_t recent,
                                                          const int32_t* __restrict__ table_out, uint32_t max_pages_out) {
     constexpr uint32_t kLanes = D / 8;                 // 16-byte pieces of a row
     constexpr uint32_t kRows = 256 / kLanes;           // rows of a CTA's step
     constexpr int kSteps = 4;
     pdl_trigger();
-    pdl_wait();
     const uint32_t unit = blockIdx.y, b = unit / c.hkv, h = unit % c.hkv;
-    const uint32_t stay = min(c.length(b), budget);
-    const uint32_t piece = threadIdx.x % kLanes, i0 = blockIdx.x * (kSteps * kRows) + threadIdx.x / kLanes;
-    if (i0 >= stay) return;
+    const uint32_t n = c.length(b), stay = min(n, budget), chosen = n <= budget ? 0 : stay - recent;     // rows the selection has to name
+    const uint32_t piece = threadIdx.x % kLanes, first = blockIdx.x * (kSteps * kRows), i0 = first + threadIdx.x / kLanes;
+    const bool early = first >= chosen;
+    if (!early || first >= stay) pdl_wait();
+    if (first >= stay) return;
     uint32_t src[kSteps], dst[kSteps];
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) src[u] = i0 + u * kRows < stay ? (uint32_t)rows_ws[(size_t)unit * budget + i0 + u * kRows] : kNoRow;
+    for (int u = 0; u < kSteps; ++u) {
+        const uint32_t i = i0 + u * kRows;
+        src[u] = i >= stay ? kNoRow : i >= chosen ? i + (n - stay) : (uint32_t)rows_ws[(size_t)unit * budget + i];
+    }
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
         dst[u] = src[u] == kNoRow ? kNoRow : c.row(table_out, max_pages_out, b, h, i0 + u * kRows);
@@ -430,6 +463,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(View c, const int32_t* 
             reinterpret_cast<uint4*>(c.k)[(size_t)dst[u] * kLanes + piece] = k[u];
             reinterpret_cast<uint4*>(c.v)[(size_t)dst[u] * kLanes + piece] = v[u];
         }
+    if (early) pdl_wait();                             // this kernel is not done before the selection is
 }
 
 // ---------------------------------------------------------------- beams take over their parents' pages
@@ -517,10 +551,12 @@ catena_status_t catena_b200_rope_append_paged_bf16_into(const catena_paged_cache
     if (!token_start && tokens != c.n_seqs) return fail(CATENA_E_BAD_ARG, "rope_append_paged: without token_start there is one token per sequence");
     CATENA_TRY(begin(&c.err));
     const bool wide = cache->head_dim == 128;
-    const uint64_t work = (n_heads + 2 * c.hkv) * (cache->head_dim / 16);
-    const dim3 grid((unsigned)tokens, (unsigned)ceil_div_u64(work, 128));
+    // CTAs of all heads of a token, or of a part of them until there are some for every SM
+    const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148, steps = ceil_div_u64((n_heads + 2 * c.hkv) * (cache->head_dim / 16), 128);
+    const uint64_t parts = ceil_div_u64(sms * 4, tokens);
+    const dim3 grid((unsigned)tokens, (unsigned)(parts < steps ? parts : steps));
     CATENA_TRY(launch("rope_append_paged_kernel", wide ? rope_append_paged_kernel<128> : rope_append_paged_kernel<64>, grid, dim3(128), 0, c,
-                      (const __nv_bfloat16*)qkv, qkv_pitch, token_start, positions, (const float2*)angles, (uint32_t)n_angles, (uint32_t)n_heads,
+                      (const __nv_bfloat16*)qkv, qkv_pitch, token_start, positions, (const float4*)angles, (uint32_t)n_angles, (uint32_t)n_heads,
                       (__nv_bfloat16*)q_out));
     return end();
 }
@@ -569,7 +605,7 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     const uint64_t rows_per_cta = 4 * (256 / (cache->head_dim / 8));
     const dim3 grid((unsigned)ceil_div_u64(budget, rows_per_cta), (unsigned)units);
     CATENA_TRY(launch("evict_copy_kernel", cache->head_dim == 128 ? evict_copy_kernel<128> : evict_copy_kernel<64>, grid, dim3(256), 0, c,
-                      (const int32_t*)workspace, (uint32_t)budget, table_out, (uint32_t)max_pages_out));
+                      (const int32_t*)workspace, (uint32_t)budget, (uint32_t)recent, table_out, (uint32_t)max_pages_out));
     return end();
 }
 
