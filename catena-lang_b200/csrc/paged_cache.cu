@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(128) rope_append_paged_kernel(View c, const __
 // leaves a bin of at most 256 rows, which are ranked by comparing them with each other; ties at the limit go to the lowest rows.
 // A NaN counts as -inf and -0 as +0, so the order is total.  What stays is then written in order: every warp counts in its part
 // of the stretch and writes once it knows how many stay before it.
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kBinsPer = kBins / kSelThreads;
@@ -586,12 +586,12 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     const uint64_t units = (uint64_t)c.n_seqs * c.hkv;
     if (units > 65535) return fail(CATENA_E_TOO_LARGE, "kv_evict_paged: more than 65535 (sequence, kv head) pairs");
     CATENA_TRY(begin(&c.err));
-    // A CTA per 1024 rows that a sequence may have, up to eight and as long as every CTA has an SM of its own.  (Clusters of small
-    // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take 17.)  The shared memory that keeps a second CTA
+    // A CTA per 2048 rows that a sequence may have, up to eight and as long as every CTA has an SM of its own.  (Clusters of small
+    // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take 16.)  The shared memory that keeps a second CTA
     // off the SM is asked for whether it is filled or not.
     const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148;
     uint32_t ctas = 1;
-    while (ctas < kMaxCluster && c.cap() > 1024u * ctas && units * ctas * 2 <= sms) ctas *= 2;
+    while (ctas < kMaxCluster && c.cap() > 2048u * ctas && units * ctas * 2 <= sms) ctas *= 2;
     const uint64_t stretch = ceil_div_u64(c.cap(), ctas * kSelWarps * 32) * (kSelWarps * 32);
     const uint32_t room = stretch > kSelRoom ? 0u : (uint32_t)stretch;
     size_t smem = (size_t)room * 4 + room / 8;
