@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kThreads) beam_stats_kernel(Rows<T> rows, uint
 // ---------------------------------------------------------------- launch 2
 constexpr int kPickThreads = 1024;
 constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kBests = 2 * kMaxK + kPickWarps;        // values among which the limit is looked for
 
 struct Total {
     uint64_t total;       // order-preserving bits of the f64 total; 0: none
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(Rows<T> rows, c
     __shared__ Beams s_beam;
     __shared__ float s_least[kMaxBeams];
     __shared__ Total cand[kRoom], per_warp[kPickWarps];
-    __shared__ __align__(16) uint32_t s_best[4 * kPickWarps];
+    __shared__ __align__(16) uint32_t s_best[kBests];
     __shared__ uint32_t s_n, s_lists, s_lim, s_first, s_off, s_list[kRoom];
     pdl_trigger();
     pdl_wait();
@@ -243,57 +244,81 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(Rows<T> rows, c
         }
     }
     if (tid == 0) {
-        s_n = s_lists = s_first = s_off = 0;
-        s_lim = 0xFFFFFFFFu;
+        s_n = s_lists = 0;
     }
     __syncthreads();
 
-    // every warp's `share` best segments, and of all of those the k-th best
-    uint32_t best = 0, best_beam = 0;
-    for (uint32_t i = seg0; i < n_segs; i += kPickThreads) {
-        const uint32_t w = i / segs, v = order_bits(__fadd_rn(i == seg0 ? x0 : st[i].x, s_beam.off[w]));
-        if (v > best) { best = v; best_beam = w; }
-    }
-    const uint32_t share = (2 * k + kPickWarps - 1) / kPickWarps;            // 1 .. 4
-    {
+    // Candidates: first a limit from the segments' maxima; if the segments that reach it hold too many logits that do (few segments,
+    // or one beam far ahead of the others), a second one from the logits of these segments.
+    const uint32_t width = rows.pieces * 32 * Rows<T>::N;
+#pragma unroll 1
+    for (int attempt = 0; attempt < 2; ++attempt) {
+        uint32_t best = 0, best_beam = 0, n = attempt == 0 ? n_segs : s_lists * width;      // of what a thread looks at; its beam
+        for (uint32_t i = attempt == 0 ? seg0 : tid; i < n; i += kPickThreads) {
+            uint32_t w;
+            float x;
+            if (attempt == 0) {
+                w = i / segs;
+                x = i == seg0 ? x0 : st[i].x;
+            } else {
+                const uint32_t nth = i / s_lists, at = s_list[i - nth * s_lists];        // neighbours look at different segments
+                w = at / segs;
+                const uint32_t token = (at - w * segs) * width + nth;
+                if (token >= rows.vocab) continue;
+                x = take(Piece<T>::one(rows.logits + (size_t)(row0 + w) * rows.pitch + token));
+            }
+            const uint32_t v = order_bits(__fadd_rn(x, s_beam.off[w]));
+            if (v > best) { best = v; best_beam = w; }
+        }
+        // the limit: of every warp's `share` best, 2 k or more in all, the k-th best
+        const uint32_t active = min((attempt == 0 ? n : (n + 31) / 32), (uint32_t)kPickWarps);
+        const uint32_t share = min(32u, (2 * k + active - 1) / active), bests = (active * share + 3) / 4 * 4;
+        for (uint32_t i = tid; i < kBests; i += kPickThreads) s_best[i] = 0;
+        __syncthreads();
+        if (tid == 0) {
+            s_first = s_off = s_n = 0;
+            s_lim = 0xFFFFFFFFu;
+        }
         uint32_t v = best;
-        for (uint32_t i = 0; i < share; ++i) {
+        for (uint32_t i = 0; i < share && warp < active; ++i) {
             const uint32_t nth = __reduce_max_sync(0xFFFFFFFFu, v);
             const uint32_t holders = __ballot_sync(0xFFFFFFFFu, v == nth);
             if (lane == (uint32_t)__ffs(holders) - 1) {
                 v = 0;
-                s_best[i * kPickWarps + warp] = nth;
+                s_best[warp * share + i] = nth;
             }
         }
-    }
-    __syncthreads();
-    if (tid < share * kPickWarps) {
-        const uint32_t mine = s_best[tid];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < share * kPickWarps; j += 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(s_best + j);
-            rank += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
+        __syncthreads();
+        if (tid < bests) {
+            const uint32_t mine = s_best[tid];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < bests; j += 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(s_best + j);
+                rank += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+            }
+            if (rank < k) atomicMin(&s_lim, mine);                // 0 when there are fewer than k: no limit
+            if (rank == 0) s_first = mine;
         }
-        if (rank < k) atomicMin(&s_lim, mine);                    // 0 when there are fewer than k: no limit
-        if (rank == 0) s_first = mine;
-    }
-    __syncthreads();
-    const uint32_t lim = s_lim;
-    if (best >= lim && best) atomicMax(&s_off, __float_as_uint(fabsf(s_beam.off[best_beam])));
-    __syncthreads();
-    if (tid < beams) {
-        const double l = value_of(lim), first = value_of(s_first), off = s_beam.off[tid], most = __uint_as_float(s_off);
-        const double least = l - off - 0x1p-20 * (fabs(l) + fabs(first) + fabs(off) + most);
-        s_least[tid] = lim && least == least ? __double2float_rd(least) : -INFINITY;
-    }
-    __syncthreads();
-    for (uint32_t i = seg0; i < n_segs; i += kPickThreads) {
-        if ((i == seg0 ? x0 : st[i].x) < s_least[i / segs]) continue;
-        const uint32_t at = atomicAdd(&s_lists, 1u);
-        if (at < kRoom) s_list[at] = i;
-    }
-    __syncthreads();
-    if (s_lists <= kRoom) {
+        __syncthreads();
+        const uint32_t lim = s_lim;
+        if (best >= lim && best) atomicMax(&s_off, __float_as_uint(fabsf(s_beam.off[best_beam])));
+        __syncthreads();
+        // the least logit of each beam that can be a candidate
+        if (tid < beams) {
+            const double l = value_of(lim), top = value_of(s_first), off = s_beam.off[tid], most = __uint_as_float(s_off);
+            const double least = l - off - 0x1p-20 * (fabs(l) + fabs(top) + fabs(off) + most);
+            s_least[tid] = lim && least == least ? __double2float_rd(least) : -INFINITY;
+        }
+        __syncthreads();
+        if (attempt == 0) {
+            for (uint32_t i = seg0; i < n_segs; i += kPickThreads) {
+                if ((i == seg0 ? x0 : st[i].x) < s_least[i / segs]) continue;
+                const uint32_t at = atomicAdd(&s_lists, 1u);
+                if (at < kRoom) s_list[at] = i;
+            }
+            __syncthreads();
+            if (s_lists > kRoom) break;
+        }
         for (uint32_t i = warp; i < s_lists; i += kPickWarps) {
             const uint32_t w = s_list[i] / segs, seg = s_list[i] - w * segs;
             const float least = s_least[w];
@@ -304,15 +329,17 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(Rows<T> rows, c
                 if (x[u] < least) continue;                       // a NaN goes on
                 const uint32_t token = rows.index(seg, u, lane);
                 if ((uint32_t)u / Rows<T>::N >= rows.pieces || token >= rows.vocab) continue;
-                const float v = take(x[u]);
                 const uint32_t at = atomicAdd(&s_n, 1u);
-                if (at < kRoom) cand[at] = {s_beam.total(w, v), key_of(v, token), w};
+                if (at < kRoom) cand[at] = {0, key_of(take(x[u]), token), w};
             }
         }
+        __syncthreads();
+        if (s_n <= kRoom) break;
     }
-    __syncthreads();
     const uint32_t n = s_n;
     if (s_lists <= kRoom && n <= kRoom) {
+        if (tid < n) cand[tid].total = s_beam.total((uint32_t)cand[tid].beam, value_of((uint32_t)(cand[tid].key >> 32)));
+        __syncthreads();
         for (uint32_t i = warp; i < n; i += kPickWarps) {         // a warp ranks a candidate
             const Total mine = cand[i];
             uint32_t place = 0;
@@ -344,7 +371,6 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(Rows<T> rows, c
     }
     __syncthreads();
     last = {~0ull, ~0ull, 0};
-    const uint32_t width = rows.pieces * 32 * Rows<T>::N;
     for (uint32_t place = 0; place < k; ++place) {
         Total mine = {0, 0, 0};
         for (uint32_t i = tid; i < lists * width; i += kPickThreads) {

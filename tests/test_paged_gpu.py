@@ -391,7 +391,7 @@ def select_reference(logits, scores, batch, beams, k):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("batch,beams,vocab,k", [(1, 1, 1, 1), (2, 4, 100, 8), (3, 1, 7, 7), (1, 4, 32000, 8), (2, 5, 50257, 10), (2, 64, 4100, 64), (1, 2, 4096, 64),
-                                                 (5, 3, 33, 64), (1, 1, 300000, 33), (40, 2, 9000, 4)])
+                                                 (5, 3, 33, 64), (1, 1, 300000, 33), (40, 2, 9000, 4), (3, 16, 200, 32), (2, 12, 64, 24), (1, 2, 300, 64)])
 @pytest.mark.parametrize("pad", [0, 3])
 def test_select(dtype, batch, beams, vocab, k, pad):
     g = torch.Generator("cuda").manual_seed(beams * 1000 + vocab)
@@ -416,6 +416,21 @@ def test_select_ties_go_to_the_lowest_beam_and_token():
     ordered = torch.arange(5000, device="cuda").float().repeat(8, 1) * 0.01     # the best all in one chunk, in ascending order
     got = select(ordered, torch.tensor([0.0, -100, -100, -100] * 2, device="cuda"), 2, 4, 64)
     assert got[2].tolist() == [list(range(4999, 4999 - 64, -1))] * 2 and (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,beams,vocab,k", [(2, 4, 32000, 8), (3, 16, 200, 32), (2, 8, 5000, 64)])
+def test_select_of_beams_of_very_different_merit(dtype, batch, beams, vocab, k):
+    """The first step of a search marks all beams but one by a large negative score; later one beam leads by far."""
+    g = torch.Generator("cuda").manual_seed(3)
+    logits = (torch.randn(batch * beams, vocab, generator=g, device="cuda") * 3).to(dtype)
+    for others in (-1e9, -math.inf, -40.0):
+        scores = torch.full((batch, beams), others, device="cuda")
+        scores[:, 1] = 0.0
+        got = select(logits, scores.view(-1), batch, beams, k)
+        value, parent, token = select_reference(logits, scores.view(-1), batch, beams, k)
+        assert torch.equal(got[1].long(), parent) and torch.equal(got[2].long(), token)
+        assert (parent == 1).all() or vocab < k
 
 
 def test_select_of_masks_and_dead_beams():
