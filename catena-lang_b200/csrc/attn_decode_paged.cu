@@ -563,7 +563,8 @@ template <int D, int NT, bool WEIGHTS>
 static catena_status_t launch_attention(const View& c, const Plan& p, const void* q, void* o, uint64_t hq, float scale, const float* weights_in,
                                         float* weights_out, uint8_t* ws) {
     auto kernel = attn_decode_paged_kernel<D, NT, WEIGHTS>;
-    CATENA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem));
+    static thread_local uint32_t told = 0;
+    CATENA_TRY(allow_smem(kernel, Shape<D>::kSmem, &told));
     Partials part = {(uint2*)(ws + p.first), (float2*)(ws + p.ml), (float*)(ws + p.o), nullptr, nullptr, nullptr, p.pitch};
     uint64_t ctas = p.ranges;
     if (WEIGHTS) {
@@ -603,7 +604,7 @@ catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache
     if (!q || !o || !workspace || (weights_in && !weights_out)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: null argument");
     if (!aligned16(q) || !aligned16(o) || !aligned4(weights_in) || !aligned4(weights_out) || ((uintptr_t)workspace & 255))
         return fail(CATENA_E_BAD_ARG, "attn_decode_paged: q and o must be 16-byte aligned, the workspace 256-byte");
-    if (scale - scale != 0.0f) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite");
+    if (!(fabsf(scale) < 1e30f)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite (below 1e30)");
     // tiles of the whole call are counted in 32 bits
     if ((uint64_t)c.n_seqs * c.hkv > 0x7FFFFFFFull || (uint64_t)c.n_seqs * c.hkv * (c.cap() / 64 + 1) > 0xFFFFFFFFull || (weights_out && (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), kWeightRows) > 0x7FFF0000ull))
         return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: more (sequence, kv head) pairs than the kernels index");

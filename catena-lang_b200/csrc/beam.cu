@@ -326,11 +326,12 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(Rows<T> rows, c
             rows.load(row0 + w, seg, lane, x);
 #pragma unroll
             for (int u = 0; u < kPer; ++u) {
-                if (x[u] < least) continue;                       // a NaN goes on
+                const float v = take(x[u]);
+                if (v < least) continue;
                 const uint32_t token = rows.index(seg, u, lane);
                 if ((uint32_t)u / Rows<T>::N >= rows.pieces || token >= rows.vocab) continue;
                 const uint32_t at = atomicAdd(&s_n, 1u);
-                if (at < kRoom) cand[at] = {0, key_of(take(x[u]), token), w};
+                if (at < kRoom) cand[at] = {0, key_of(v, token), w};
             }
         }
         __syncthreads();
@@ -423,6 +424,7 @@ static catena_status_t select_into(const T* logits, uint64_t pitch, const float*
     rows.segs = (uint32_t)ceil_div_u64(vocab, rows.pieces * 32 * Piece<T>::kN);
     rows.vec = paged::aligned16(logits) && pitch * sizeof(T) % 16 == 0;
     const uint64_t n = batch * beams * rows.segs;
+    if (ceil_div_u64(n, kWarps) > 0x7FFFFFFFull) return fail(CATENA_E_TOO_LARGE, "beam_select: more logits than the kernels index");
     float2* stats = static_cast<float2*>(workspace);
     CATENA_TRY(paged::launch("beam_stats_kernel", beam_stats_kernel<T>, dim3((unsigned)ceil_div_u64(n, kWarps)), dim3(kThreads), 0, rows, n, stats));
     CATENA_TRY(paged::launch("beam_pick_kernel", beam_pick_kernel<T>, dim3((unsigned)batch), dim3(kPickThreads), 0, rows, stats, scores, (uint32_t)beams,

@@ -52,13 +52,15 @@ static catena_status_t bind_device(int device) {
     if (device < 0 || device >= count) return fail(CATENA_E_BAD_ARG, "device index out of range");
     if (device >= kMaxDevices) return fail(CATENA_E_UNSUPPORTED, "device index beyond the 16 devices the per-device tables hold");
     CATENA_CUDA(cudaSetDevice(device));
-    cudaDeviceProp prop;
-    CATENA_CUDA(cudaGetDeviceProperties(&prop, device));
-    if (prop.major != 10)
+    // two attributes; cudaGetDeviceProperties would fetch everything there is to know, which takes a millisecond
+    int major = 0, sms = 0;
+    CATENA_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    CATENA_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    if (major != 10)
         return fail(CATENA_E_NO_DEVICE, "kernels are built for sm_100a only (Blackwell B200)");
     g_tls.device = device;
-    g_tls.sm_count = prop.multiProcessorCount;
-    g_tls.cc_major = prop.major;
+    g_tls.sm_count = sms;
+    g_tls.cc_major = major;
     return CATENA_OK;
 }
 

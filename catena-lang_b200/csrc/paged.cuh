@@ -62,6 +62,16 @@ static inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Lets a kernel have `bytes` of dynamic shared memory; `done` belongs to the kernel (a bit per device that has been told).
+template <class F>
+static catena_status_t allow_smem(F kernel, size_t bytes, uint32_t* done) {
+    const uint32_t bit = 1u << tls().device;
+    if (*done & bit) return CATENA_OK;
+    CATENA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    *done |= bit;
+    return CATENA_OK;
+}
+
 struct How {
     uint32_t cluster = 1;
     bool early = true;      // may start while the launch before it still runs

@@ -596,7 +596,8 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     const uint32_t room = stretch > kSelRoom ? 0u : (uint32_t)stretch;
     size_t smem = (size_t)room * 4 + room / 8;
     if (ctas > 1 && smem < kSelAlone) smem = kSelAlone;
-    if (smem > 32768) CATENA_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelRoom * 4 + kSelRoom / 8));
+    static thread_local uint32_t told = 0;
+    CATENA_TRY(allow_smem(evict_select_kernel, kSelRoom * 4 + kSelRoom / 8, &told));
     How how;
     how.cluster = ctas;
     CATENA_TRY(launch_as(how, "evict_select_kernel", evict_select_kernel, dim3((unsigned)units * ctas), dim3(kSelThreads), smem, c, weights,

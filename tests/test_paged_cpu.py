@@ -68,7 +68,7 @@ def test_null_cache():
 @pytest.mark.parametrize("change,status", [
     (dict(q=None), cb.E_BAD_ARG), (dict(o=None), cb.E_BAD_ARG), (dict(ws=None), cb.E_BAD_ARG), (dict(q=A + 8), cb.E_BAD_ARG), (dict(o=A + 2), cb.E_BAD_ARG),
     (dict(ws=A + 16), cb.E_BAD_ARG), (dict(heads=3), cb.E_UNSUPPORTED), (dict(heads=0), cb.E_UNSUPPORTED), (dict(heads=34), cb.E_UNSUPPORTED),
-    (dict(scale=float("nan")), cb.E_BAD_ARG), (dict(scale=float("inf")), cb.E_BAD_ARG), (dict(w_in=A), cb.E_BAD_ARG), (dict(w_out=A + 1), cb.E_BAD_ARG)])
+    (dict(scale=float("nan")), cb.E_BAD_ARG), (dict(scale=float("inf")), cb.E_BAD_ARG), (dict(scale=-3e38), cb.E_BAD_ARG), (dict(w_in=A), cb.E_BAD_ARG), (dict(w_out=A + 1), cb.E_BAD_ARG)])
 def test_attention_refusals(change, status):
     assert attend(**change) == status
 

@@ -449,6 +449,12 @@ def test_select_of_masks_and_dead_beams():
     got = select(logits[:2, :4], torch.tensor([0.0, -inf], device="cuda"), 1, 2, 8)      # nothing is left: -inf, in order
     by_logit = logits[1, :4].sort(descending=True).indices.tolist()
     assert (got[0] == -inf).all() and got[1].tolist() == [[0] * 4 + [1] * 4] and got[2].tolist() == [[0, 1, 2, 3] + by_logit]
+    holes = torch.randn(2, 5000, generator=g, device="cuda")
+    holes[:, ::2] = math.nan                             # half of everything
+    got = select(holes, torch.zeros(2, device="cuda"), 1, 2, 6)
+    value, parent, token = select_reference(holes, torch.zeros(2, device="cuda"), 1, 2, 6)
+    assert torch.equal(got[1].long(), parent) and torch.equal(got[2].long(), token)
+    assert ((got[0].double() - value).abs() <= 1e-5).all()
     big = torch.zeros(1, 10, device="cuda")
     big[0, 3] = inf
     got = select(big, torch.zeros(1, device="cuda"), 1, 1, 2)
@@ -533,6 +539,43 @@ def test_a_captured_step_replays_on_new_lengths_and_two_streams_do_not_meet():
     o_ref, off, _, _ = attention_reference(c, q, 0.09, 1, int(c.lengths[1]))
     assert ((o[1].double() - o_ref).abs() <= 2.0 ** -8 * o_ref.abs() + off * (1 + 2.0 ** -8)).all()
     cb.check(L.catena_b200_check_device_errors())
+
+
+def test_two_host_threads_on_streams_of_their_own():
+    """Library state belongs to the thread: calls that overlap on the device, each with its own workspace, give the bits of calls alone."""
+    import threading
+    L = cb.lib()
+    caches = [Cache(20 + i, [700, 3, 0, 1500, 64], 4, 128, 16, spare=40) for i in range(2)]
+    qs = [torch.randn(5, 8, 128, generator=c.gen, device="cuda").bfloat16() for c in caches]
+    want = [attend(c, q, 0.1)[1] for c, q in zip(caches, qs)]
+    logits = [torch.randn(8, 20000, generator=c.gen, device="cuda") for c in caches]
+    picked = [select(x, torch.zeros(8, device="cuda"), 2, 4, 8) for x in logits]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            cb.check(L.catena_b200_init(0))
+            stream = torch.cuda.Stream()
+            cb.check(L.catena_b200_set_stream(stream.cuda_stream))
+            L.catena_b200_set_blocking(0)
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    status, got = attend(caches[i], qs[i], 0.1)
+                    cb.check(status)
+                    again = select(logits[i], torch.zeros(8, device="cuda"), 2, 4, 8)
+                    stream.synchronize()
+                    if not torch.equal(got, want[i]) or not all(torch.equal(a, b) for a, b in zip(again, picked[i])):
+                        wrong.append(i)
+            cb.check(L.catena_b200_check_device_errors())
+        except Exception as exc:          # noqa: BLE001 - reported below
+            wrong.append(repr(exc))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_a_serving_run():
