@@ -425,13 +425,15 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(View c, const
 
 // ---------------------------------------------------------------- eviction: the rows that stay, into their new pages
 // The recent rows stay whatever the weights are, and all rows of a sequence within its budget: CTAs that have only such rows copy
-// while the selection still runs (which starts them only once everything before it is done).
+// while the selection still runs (which starts them only once everything before it is done).  Bound by the chain row number -> page
+// -> data: two rows per thread on 64 warps per SM took 29.6 us with the selection (4 x 16384 rows), four on 32 warps 30.8.
+constexpr int kCopySteps = 2;
 template <int D>
-__global__ void __launch_bounds__(256) evict_copy_kernel(View c, const int32_t* rows_ws, uint32_t budget, uint32_t recent,
+__global__ void __launch_bounds__(256, 8) evict_copy_kernel(View c, const int32_t* rows_ws, uint32_t budget, uint32_t recent,
                                                          const int32_t* __restrict__ table_out, uint32_t max_pages_out) {
     constexpr uint32_t kLanes = D / 8;                 // 16-byte pieces of a row
     constexpr uint32_t kRows = 256 / kLanes;           // rows of a CTA's step
-    constexpr int kSteps = 4;
+    constexpr int kSteps = kCopySteps;
     pdl_trigger();
     const uint32_t unit = blockIdx.y, b = unit / c.hkv, h = unit % c.hkv;
     const uint32_t n = c.length(b), stay = min(n, budget), chosen = n <= budget ? 0 : stay - recent;     // rows the selection has to name
@@ -500,6 +502,7 @@ __global__ void __launch_bounds__(128) beam_reorder_kernel(View c, const int32_t
             if (tid == 0) atomicOr(c.err, kErrTable);
         } else {
             const size_t src = ((size_t)from * c.hkv + h) * c.page_size * (D / 8), dst = ((size_t)to * c.hkv + h) * c.page_size * (D / 8);
+#pragma unroll 4
             for (uint32_t i = tid; i < rest * (D / 8); i += 128) {
                 const uint4 k = reinterpret_cast<const uint4*>(c.k)[src + i], v = reinterpret_cast<const uint4*>(c.v)[src + i];
                 reinterpret_cast<uint4*>(c.k)[dst + i] = k;
@@ -510,6 +513,7 @@ __global__ void __launch_bounds__(128) beam_reorder_kernel(View c, const int32_t
     if (weights) {
         const float* w = weights + ((size_t)p * c.hkv + h) * c.cap();
         float* o = weights_out + ((size_t)s * c.hkv + h) * c.cap();
+#pragma unroll 8
         for (uint32_t i = tid; i < c.cap(); i += 128) o[i] = i < n ? w[i] : 0.0f;
     }
 }
@@ -603,7 +607,7 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     CATENA_TRY(launch_as(how, "evict_select_kernel", evict_select_kernel, dim3((unsigned)units * ctas), dim3(kSelThreads), smem, c, weights,
                               (uint32_t)budget, (uint32_t)recent, lengths_out, weights_out, (uint32_t)(max_pages_out * c.page_size), kept,
                               (int32_t*)workspace, room));
-    const uint64_t rows_per_cta = 4 * (256 / (cache->head_dim / 8));
+    const uint64_t rows_per_cta = kCopySteps * (256 / (cache->head_dim / 8));
     const dim3 grid((unsigned)ceil_div_u64(budget, rows_per_cta), (unsigned)units);
     CATENA_TRY(launch("evict_copy_kernel", cache->head_dim == 128 ? evict_copy_kernel<128> : evict_copy_kernel<64>, grid, dim3(256), 0, c,
                       (const int32_t*)workspace, (uint32_t)budget, (uint32_t)recent, table_out, (uint32_t)max_pages_out));
