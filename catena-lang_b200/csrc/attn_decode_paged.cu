@@ -40,7 +40,7 @@ template <int D> struct Shape {
     static constexpr int kPitch = D + 4;                      // floats per head of the merge buffer: conflict-free for (8 d, 4 heads)
     static constexpr uint32_t kRing = kWarps * kWarpBytes;
     static constexpr uint32_t kMerge = kWarps * 8 * kPitch * 4;
-    static constexpr uint32_t kSmem = kRing + kMerge + kWarps * 8 * 2 * 4;
+    static constexpr uint32_t kSmem = kRing + kMerge;
 };
 
 // The tiles in `ranges` ranges, of which the first `tiles` have one each when there are fewer.  start(k) = k tiles / n, in 32 bits.
@@ -120,6 +120,14 @@ struct Cursor {
     }
 };
 
+// four elements of an output: sum / L, zeros where no row has any weight
+__device__ __forceinline__ void store_o(__nv_bfloat16* o, const float4& sum, float L) {
+    const float r = __frcp_rn(L);
+    __nv_bfloat162 lo = __floats2bfloat162_rn(__fmul_rn(sum.x, r), __fmul_rn(sum.y, r)), hi = __floats2bfloat162_rn(__fmul_rn(sum.z, r), __fmul_rn(sum.w, r));
+    if (L == 0.0f) lo = hi = __floats2bfloat162_rn(0.0f, 0.0f);
+    *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
 template <int D, int NT, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_kernel(View c, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ o,
                                                                                  uint32_t hq, float scale_log2, Partials part) {
@@ -127,7 +135,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
     constexpr int KEYS = S::kKeys, TILE = S::kTile, SUB = KEYS / 16, CH = D / 8;     // CH: 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t smem[];
     float* merge = reinterpret_cast<float*>(smem + S::kRing);
-    float2* merge_ml = reinterpret_cast<float2*>(smem + S::kRing + S::kMerge);
+    // the maxima are written before a segment's first barrier, while a slow warp may still read the last segment's: two of them in turn
+    __shared__ float merge_ms[2][kWarps][NT * 8], merge_l[kWarps][NT * 8];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const uint32_t group = hq / c.hkv, range = blockIdx.x;
     pdl_trigger();
@@ -212,7 +221,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
 
     uint32_t qf[NT][D / 16][2];
     float acc[NT][D / 16][4], m[NT][2], l[NT][2];
+    // the group's queries for a segment, as the second operand of the products with the keys
+    auto load_q = [&](uint32_t b, uint32_t h) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t head = nt * 8 + g;
+            const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + ((size_t)b * hq + h * group + (head < group ? head : 0)) * D);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                qf[nt][kk][0] = head < group ? qr[kk * 8 + t4] : 0u;
+                qf[nt][kk][1] = head < group ? qr[kk * 8 + 4 + t4] : 0u;
+            }
+        }
+    };
     look_up();
+    load_q(at.b, at.h);
     uint32_t row = next_row();
     issue(c.k, row, kbase);
     issue(c.v, row, vbase);
@@ -220,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
     write_zeros();
 
     uint32_t seg_first = 0;
+    uint32_t turn = 0;
     bool fresh = true;                                             // the next tile begins a segment
     for (uint32_t t = t0; t < t1; ++t) {
         if (fresh) {
@@ -227,14 +251,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
             seg_first = at.tile;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t head = nt * 8 + g;
-                const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + ((size_t)at.b * hq + at.h * group + (head < group ? head : 0)) * D);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    qf[nt][kk][0] = head < group ? qr[kk * 8 + t4] : 0u;
-                    qf[nt][kk][1] = head < group ? qr[kk * 8 + 4 + t4] : 0u;
-                    for (int e = 0; e < 4; ++e) acc[nt][kk][e] = 0.0f;
-                }
+                for (int mt = 0; mt < D / 16; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.0f;
                 m[nt][0] = m[nt][1] = -INFINITY;
                 l[nt][0] = l[nt][1] = 0.0f;
             }
@@ -263,12 +281,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
         row = next_row();
         issue(c.k, row, kbase);
         look_up();
+        const Cursor<TILE> now = at;
+        at.next(c);
+        if (at.tile == 0 && t + 1 < t1) load_q(at.b, at.h);        // the next segment's, while this one is finished
         // thread: keys g, g + 8 of every 16 (rows of s), heads 2 t4, 2 t4 + 1 of each n-tile
         bool raise = false;
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
             const uint32_t key = r0 + sub * 16 + g;
-            const bool live0 = key < at.n, live1 = key + 8 < at.n;
+            const bool live0 = key < now.n, live1 = key + 8 < now.n;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -281,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
                     if (WEIGHTS) {
                         const uint32_t head = nt * 8 + 2 * t4 + e;
                         if (head < group) {
-                            float* dst = part.scores + ((size_t)at.b * hq + at.h * group + head) * part.pitch;
+                            float* dst = part.scores + ((size_t)now.b * hq + now.h * group + head) * part.pitch;
                             if (live0) dst[key] = s0;
                             if (live1) dst[key + 8] = s1;
                         }
@@ -350,52 +371,65 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
         __syncwarp();
         issue(c.v, row, vbase);
 
-        const uint32_t unit_tiles = at.tiles(), b = at.b, h = at.h, tile = at.tile;
-        at.next(c);
+        const uint32_t unit_tiles = now.tiles(), b = now.b, h = now.h, tile = now.tile;
         if (at.tile != 0 && t + 1 < t1) continue;
         // ---- the segment [seg_first, tile] of unit (b, h) is done: join the warps
         fresh = true;
         const bool whole = seg_first == 0 && tile + 1 == unit_tiles;
         const uint32_t slot = range * 2 + (seg_first == 0 ? 1u : 0u);
+        float (&merge_m)[kWarps][NT * 8] = merge_ms[turn];
+        turn ^= 1;
+        // first the common maximum, then every warp's part at that scale, then sums of four: the exponentials are taken once
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) l[nt][e] = __fadd_rn(l[nt][e], __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], off));
+                if (g == 0) merge_m[warp][nt * 8 + 2 * t4 + e] = m[nt][e];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t j = nt * 8 + 2 * t4 + e;
+                const float M = fmaxf(fmaxf(merge_m[0][j], merge_m[1][j]), fmaxf(merge_m[2][j], merge_m[3][j]));
+                const float f = m[nt][e] == M ? 1.0f : ex2(__fsub_rn(m[nt][e], M));
+                if (g == 0) merge_l[warp][j] = __fmul_rn(l[nt][e], f);
                 float* dst = merge + (warp * 8 + 2 * t4 + e) * S::kPitch + g;
 #pragma unroll
                 for (int mt = 0; mt < D / 16; ++mt) {
-                    dst[mt * 16] = acc[nt][mt][e];
-                    dst[mt * 16 + 8] = acc[nt][mt][2 + e];
+                    dst[mt * 16] = __fmul_rn(acc[nt][mt][e], f);
+                    dst[mt * 16 + 8] = __fmul_rn(acc[nt][mt][2 + e], f);
                 }
-                if (g == 0) merge_ml[warp * 8 + 2 * t4 + e] = make_float2(m[nt][e], l[nt][e]);
             }
             __syncthreads();
-            for (uint32_t i = tid; i < 8 * D; i += kThreads) {
-                const uint32_t j = i / D, d = i % D, head = nt * 8 + j;
+            for (uint32_t i = tid; i < 8 * (D / 4); i += kThreads) {
+                const uint32_t head = nt * 8 + i / (D / 4), d4 = i % (D / 4);
                 if (head >= group) break;
-                float M = merge_ml[j].x;
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, merge_ml[w * 8 + j].x);
-                float L = 0.0f, O = 0.0f;
+                const float L = __fadd_rn(__fadd_rn(merge_l[0][head], merge_l[1][head]), __fadd_rn(merge_l[2][head], merge_l[3][head]));
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const float2 ml = merge_ml[w * 8 + j];
-                    const float f = ml.x == M ? 1.0f : ex2(__fsub_rn(ml.x, M));
-                    L = __fmaf_rn(ml.y, f, L);
-                    O = __fmaf_rn(merge[(w * 8 + j) * S::kPitch + d], f, O);
+                    const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + i / (D / 4)) * S::kPitch + d4 * 4);
+                    sum.x = __fadd_rn(sum.x, v.x);
+                    sum.y = __fadd_rn(sum.y, v.y);
+                    sum.z = __fadd_rn(sum.z, v.z);
+                    sum.w = __fadd_rn(sum.w, v.w);
                 }
+                const float M = fmaxf(fmaxf(merge_m[0][head], merge_m[1][head]), fmaxf(merge_m[2][head], merge_m[3][head]));
                 const size_t out_head = (size_t)b * hq + h * group + head;
                 if (whole) {
-                    o[out_head * D + d] = __float2bfloat16_rn(L == 0.0f ? 0.0f : __fdiv_rn(O, L));
-                    if (WEIGHTS && d == 0) part.stats[out_head] = make_float2(M, L);
+                    store_o(o + out_head * D + d4 * 4, sum, L);
+                    if (WEIGHTS && d4 == 0) part.stats[out_head] = make_float2(M, L);
                 } else {
-                    part.o[((size_t)slot * group + head) * D + d] = O;
-                    if (d == 0) part.ml[slot * 16 + head] = make_float2(M, L);
+                    reinterpret_cast<float4*>(part.o)[((size_t)slot * group + head) * (D / 4) + d4] = sum;
+                    if (d4 == 0) part.ml[slot * 16 + head] = make_float2(M, L);
                 }
             }
-            __syncthreads();
+            if (nt + 1 < NT) __syncthreads();
         }
         if (tid == 0) {
             const bool begun = !whole && seg_first == 0;               // then this is the range's last tile
@@ -408,57 +442,66 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// CTAs below `ranges` join the parts of a unit that was cut: CTA k does it for the unit that range k began and did not finish.
+// The first ranges * ceil(group / heads_each) CTAs join the parts of a unit that was cut, for heads_each of its heads: that of
+// range k does it for the unit that range k began and did not finish.  (heads_each is small where units are cut into many parts:
+// one CTA for 16 heads of a unit in 296 parts read 2.4 MB by itself and took over 100 us.)
 // The other CTAs (only with weights) do weights_out[j] = weights_in[j] + sum over the group's heads, ascending, of exp2(s_j - M) / L
 // for kWeightRows rows of a unit; they join (M, L) of a cut unit for themselves.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kWeightRows = kJoinThreads * 4;
 
-// M and L of the group's heads over slots k (+ 1 of the first) .. last, to s_m and s_l; whole CTA
-__device__ __forceinline__ void join_stats(const Partials& part, uint32_t k, uint32_t last, uint32_t group, float (*s_part)[16], float* s_m, float* s_l) {
-    const uint32_t head = threadIdx.x & 15, lane16 = threadIdx.x >> 4;           // 16 threads per head
-    float m = -INFINITY;
-    if (head < group)
-        for (uint32_t s = k + lane16; s <= last; s += kJoinThreads / 16) m = fmaxf(m, part.ml[(s * 2 + (s == k)) * 16 + head].x);
-    s_part[lane16][head] = m;
+// M and L of heads head0 .. head0 + heads - 1 over slots k (+ 1 of the first) .. last, to s_m and s_l; whole CTA
+__device__ __forceinline__ void join_stats(const Partials& part, uint32_t k, uint32_t last, uint32_t head0, uint32_t heads, float (*s_part)[16], float* s_m,
+                                           float* s_l) {
+    uint32_t wide = 1;                                     // threads are dealt to the heads in turn
+    while (wide < heads) wide *= 2;
+    const uint32_t head = threadIdx.x % wide, step = kJoinThreads / wide, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool mine = head < heads;
+    float m = -INFINITY, l = 0.0f;
+    if (mine)
+#pragma unroll 4
+        for (uint32_t s = k + threadIdx.x / wide; s <= last; s += step) m = fmaxf(m, part.ml[(s * 2 + (s == k)) * 16 + head0 + head].x);
+    for (uint32_t off = wide; off < 32; off *= 2) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+    if (lane < wide) s_part[warp][lane] = m;
     __syncthreads();
-    if (threadIdx.x < 16) {
-        for (int i = 1; i < kJoinThreads / 16; ++i) m = fmaxf(m, s_part[i][head]);
-        s_m[head] = m;
-    }
+    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, s_part[w][head]);
     __syncthreads();
-    m = s_m[head];
-    float l = 0.0f;
-    if (head < group)
-        for (uint32_t s = k + lane16; s <= last; s += kJoinThreads / 16) {
-            const float2 ml = part.ml[(s * 2 + (s == k)) * 16 + head];
+    if (mine)
+#pragma unroll 4
+        for (uint32_t s = k + threadIdx.x / wide; s <= last; s += step) {
+            const float2 ml = part.ml[(s * 2 + (s == k)) * 16 + head0 + head];
             l = __fmaf_rn(ml.y, ml.x == m ? 1.0f : ex2(__fsub_rn(ml.x, m)), l);
         }
-    s_part[lane16][head] = l;
+    for (uint32_t off = wide; off < 32; off *= 2) l = __fadd_rn(l, __shfl_xor_sync(0xFFFFFFFFu, l, off));
+    if (lane < wide) s_part[warp][lane] = l;
     __syncthreads();
-    if (threadIdx.x < 16) {
-        for (int i = 1; i < kJoinThreads / 16; ++i) l = __fadd_rn(l, s_part[i][head]);
+    if (threadIdx.x < wide) {
+        l = s_part[0][head];
+        for (int w = 1; w < kJoinWarps; ++w) l = __fadd_rn(l, s_part[w][head]);
+        s_m[head] = m;
         s_l[head] = l;
     }
     __syncthreads();
 }
 
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(View c, __nv_bfloat16* __restrict__ o, uint32_t hq, uint32_t ranges, Partials part,
-                                                                              const float* weights_in, float* weights_out) {
-    __shared__ float s_part[kJoinThreads / 16][16], s_m[16], s_l[16];
+__global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(View c, __nv_bfloat16* __restrict__ o, uint32_t hq, uint32_t ranges, uint32_t heads_each,
+                                                                              Partials part, const float* weights_in, float* weights_out) {
+    __shared__ float s_part[kJoinWarps][16], s_m[16], s_l[16];
     __shared__ float4 s_o[kJoinThreads];
     pdl_trigger();
     pdl_wait();
     const uint32_t tid = threadIdx.x, group = hq / c.hkv;
-    if (blockIdx.x < ranges) {
-        const uint32_t k = blockIdx.x;
+    const uint32_t slices = (group + heads_each - 1) / heads_each;
+    if (blockIdx.x < ranges * slices) {
+        const uint32_t k = blockIdx.x / slices, head0 = (blockIdx.x - k * slices) * heads_each, heads = min(heads_each, group - head0);
         const uint2 f = part.first[k];
         if (f.x == 0) return;
         const uint32_t last = f.x, b = f.y / c.hkv, h = f.y % c.hkv;
-        join_stats(part, k, last, group, s_part, s_m, s_l);
+        join_stats(part, k, last, head0, heads, s_part, s_m, s_l);
         // a thread has four elements of a head; where the group has few heads, several threads share the parts of one
-        const uint32_t items = group * (D / 4), team = items < kJoinThreads ? kJoinThreads / items : 1;
+        const uint32_t items = heads * (D / 4), team = items < kJoinThreads ? kJoinThreads / items : 1;
         for (uint32_t i0 = 0; i0 < items; i0 += kJoinThreads) {
             const uint32_t item = i0 + tid % min(items, (uint32_t)kJoinThreads), member = tid / min(items, (uint32_t)kJoinThreads);
             const uint32_t head = item / (D / 4), d4 = item % (D / 4);
@@ -468,8 +511,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(Vi
 #pragma unroll 4
                 for (uint32_t s = k + member; s <= last; s += team) {
                     const uint32_t slot = s * 2 + (s == k);
-                    const float m = part.ml[slot * 16 + head].x, w = m == M ? 1.0f : ex2(__fsub_rn(m, M));
-                    const float4 v = reinterpret_cast<const float4*>(part.o)[(slot * group + head) * (D / 4) + d4];
+                    const float m = part.ml[slot * 16 + head0 + head].x, w = m == M ? 1.0f : ex2(__fsub_rn(m, M));
+                    const float4 v = reinterpret_cast<const float4*>(part.o)[(slot * group + head0 + head) * (D / 4) + d4];
                     sum.x = __fmaf_rn(v.x, w, sum.x);
                     sum.y = __fmaf_rn(v.y, w, sum.y);
                     sum.z = __fmaf_rn(v.z, w, sum.z);
@@ -487,22 +530,18 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(Vi
                     sum.z = __fadd_rn(sum.z, v.z);
                     sum.w = __fadd_rn(sum.w, v.w);
                 }
-                const float L = s_l[head], r = L == 0.0f ? 0.0f : __frcp_rn(L);
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(L == 0.0f ? 0.0f : __fmul_rn(sum.x, r), L == 0.0f ? 0.0f : __fmul_rn(sum.y, r));
-                const __nv_bfloat162 hi = __floats2bfloat162_rn(L == 0.0f ? 0.0f : __fmul_rn(sum.z, r), L == 0.0f ? 0.0f : __fmul_rn(sum.w, r));
-                const size_t at = ((size_t)b * hq + h * group + head) * D + d4 * 4;
-                *reinterpret_cast<uint2*>(o + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                store_o(o + ((size_t)b * hq + h * group + head0 + head) * D + d4 * 4, sum, s_l[head]);
             }
         }
         return;
     }
-    const uint32_t blocks = (c.cap() + kWeightRows - 1) / kWeightRows, at = blockIdx.x - ranges;
+    const uint32_t blocks = (c.cap() + kWeightRows - 1) / kWeightRows, at = blockIdx.x - ranges * slices;
     const uint32_t unit = at / blocks, j0 = at % blocks * kWeightRows, b = unit / c.hkv;
     const uint32_t n = c.length(b);
     if (j0 >= n) return;
     const uint2 cut = part.split[unit];
     if (cut.x <= cut.y) {
-        join_stats(part, cut.x, cut.y, group, s_part, s_m, s_l);
+        join_stats(part, cut.x, cut.y, 0, group, s_part, s_m, s_l);
     } else if (tid < group) {
         const float2 ml = part.stats[(size_t)unit * group + tid];
         s_m[tid] = ml.x;
@@ -566,6 +605,8 @@ static catena_status_t launch_attention(const View& c, const Plan& p, const void
     static thread_local uint32_t told = 0;
     CATENA_TRY(allow_smem(kernel, Shape<D>::kSmem, &told));
     Partials part = {(uint2*)(ws + p.first), (float2*)(ws + p.ml), (float*)(ws + p.o), nullptr, nullptr, nullptr, p.pitch};
+    // eight parts per unit or more: a CTA per head
+    const uint32_t group = (uint32_t)hq / c.hkv, heads_each = (uint64_t)c.n_seqs * c.hkv * 8 < p.ranges ? 1 : group;
     uint64_t ctas = p.ranges;
     if (WEIGHTS) {
         part.split = (uint2*)(ws + p.split);
@@ -578,9 +619,10 @@ static catena_status_t launch_attention(const View& c, const Plan& p, const void
     how.early = false;
     CATENA_TRY(launch_as(how, "attn_decode_paged_kernel", kernel, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, c, (const __nv_bfloat16*)q,
                       (__nv_bfloat16*)o, (uint32_t)hq, scale * 1.44269504088896340736f, part));
+    ctas *= (group + heads_each - 1) / heads_each;
     if (WEIGHTS) ctas += (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), kWeightRows);
     return launch("attn_decode_paged_join_kernel", attn_decode_paged_join_kernel<D>, dim3((unsigned)ctas), dim3(kJoinThreads), 0, c, (__nv_bfloat16*)o,
-                  (uint32_t)hq, p.ranges, part, weights_in, weights_out);
+                  (uint32_t)hq, p.ranges, heads_each, part, weights_in, weights_out);
 }
 
 }  // namespace paged
