@@ -136,6 +136,30 @@ extern "C" {
     pub fn catena_b200_llama_decode(blk: *const catena_llama_block_t, ids: *const i32, batch: u64, pos: u64,
                                     k_cache: *mut c_void, v_cache: *mut c_void, out: *mut c_void, workspace: *mut c_void,
                                     workspace_bytes: u64) -> catena_status_t;
+
+    // key/value cache in pages, beam search
+    pub fn catena_b200_rope_angles_f32_into(base: f32, pos0: u64, count: u64, head_dim: u64, angles: *mut c_void) -> i32;
+    pub fn catena_b200_rope_append_paged_bf16_into(cache: *const catena_paged_cache_t, qkv: *const c_void, qkv_pitch: u64,
+                                                   token_start: *const i32, tokens: u64, positions: *const i32, angles: *const c_void,
+                                                   n_angles: u64, n_heads: u64, q_out: *mut c_void) -> i32;
+    pub fn catena_b200_attn_decode_paged_workspace_bytes(cache: *const catena_paged_cache_t, n_heads: u64, weights: i32) -> u64;
+    pub fn catena_b200_attn_decode_paged_bf16_into(cache: *const catena_paged_cache_t, q: *const c_void, o: *mut c_void, n_heads: u64,
+                                                   scale: f32, weights_in: *const f32, weights_out: *mut f32, workspace: *mut c_void,
+                                                   workspace_bytes: u64) -> i32;
+    pub fn catena_b200_kv_evict_paged_workspace_bytes(cache: *const catena_paged_cache_t, budget: u64) -> u64;
+    pub fn catena_b200_kv_evict_paged_bf16_into(cache: *const catena_paged_cache_t, weights: *const f32, budget: u64, recent: u64,
+                                                table_out: *const i32, max_pages_out: u64, lengths_out: *mut i32, weights_out: *mut f32,
+                                                kept: *mut i32, workspace: *mut c_void, workspace_bytes: u64) -> i32;
+    pub fn catena_b200_beam_select_workspace_bytes(batch: u64, beams: u64, vocab: u64, k: u64) -> u64;
+    pub fn catena_b200_beam_select_f32_into(logits: *const f32, pitch: u64, scores: *const f32, batch: u64, beams: u64, vocab: u64, k: u64,
+                                            out_scores: *mut f32, out_parents: *mut i32, out_tokens: *mut i32, workspace: *mut c_void,
+                                            workspace_bytes: u64) -> i32;
+    pub fn catena_b200_beam_select_bf16_into(logits: *const c_void, pitch: u64, scores: *const f32, batch: u64, beams: u64, vocab: u64,
+                                             k: u64, out_scores: *mut f32, out_parents: *mut i32, out_tokens: *mut i32,
+                                             workspace: *mut c_void, workspace_bytes: u64) -> i32;
+    pub fn catena_b200_beam_reorder_paged_bf16_into(cache: *const catena_paged_cache_t, parents: *const i32, beams: u64,
+                                                    fresh_pages: *const i32, table_out: *mut i32, lengths_out: *mut i32,
+                                                    weights: *const f32, weights_out: *mut f32) -> i32;
     pub fn catena_b200_linear_bf16_into(x: *const c_void, w: *const c_void, residual: *const c_void, y: *mut c_void, m: u64,
                                         n: u64, k: u64) -> catena_status_t;
 
@@ -178,4 +202,20 @@ pub struct catena_llama_block_t {
     pub w_gate_up: *const c_void,
     pub w_down: *const c_void,
     pub rope_base: f32,
+}
+
+/// catena_paged_cache_t of include/catena_b200.h.
+#[repr(C)]
+#[allow(non_camel_case_types)]
+pub struct catena_paged_cache_t {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub table: *const i32,
+    pub lengths: *const i32,
+    pub n_pages: u64,
+    pub page_size: u64,
+    pub n_seqs: u64,
+    pub max_pages: u64,
+    pub n_kv_heads: u64,
+    pub head_dim: u64,
 }
