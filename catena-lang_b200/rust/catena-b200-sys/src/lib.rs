@@ -138,28 +138,28 @@ extern "C" {
                                     workspace_bytes: u64) -> catena_status_t;
 
     // key/value cache in pages, beam search
-    pub fn catena_b200_rope_angles_f32_into(base: f32, pos0: u64, count: u64, head_dim: u64, angles: *mut c_void) -> i32;
+    pub fn catena_b200_rope_angles_f32_into(base: f32, pos0: u64, count: u64, head_dim: u64, angles: *mut c_void) -> catena_status_t;
     pub fn catena_b200_rope_append_paged_bf16_into(cache: *const catena_paged_cache_t, qkv: *const c_void, qkv_pitch: u64,
                                                    token_start: *const i32, tokens: u64, positions: *const i32, angles: *const c_void,
-                                                   n_angles: u64, n_heads: u64, q_out: *mut c_void) -> i32;
+                                                   n_angles: u64, n_heads: u64, q_out: *mut c_void) -> catena_status_t;
     pub fn catena_b200_attn_decode_paged_workspace_bytes(cache: *const catena_paged_cache_t, n_heads: u64, weights: i32) -> u64;
     pub fn catena_b200_attn_decode_paged_bf16_into(cache: *const catena_paged_cache_t, q: *const c_void, o: *mut c_void, n_heads: u64,
                                                    scale: f32, weights_in: *const f32, weights_out: *mut f32, workspace: *mut c_void,
-                                                   workspace_bytes: u64) -> i32;
+                                                   workspace_bytes: u64) -> catena_status_t;
     pub fn catena_b200_kv_evict_paged_workspace_bytes(cache: *const catena_paged_cache_t, budget: u64) -> u64;
     pub fn catena_b200_kv_evict_paged_bf16_into(cache: *const catena_paged_cache_t, weights: *const f32, budget: u64, recent: u64,
                                                 table_out: *const i32, max_pages_out: u64, lengths_out: *mut i32, weights_out: *mut f32,
-                                                kept: *mut i32, workspace: *mut c_void, workspace_bytes: u64) -> i32;
+                                                kept: *mut i32, workspace: *mut c_void, workspace_bytes: u64) -> catena_status_t;
     pub fn catena_b200_beam_select_workspace_bytes(batch: u64, beams: u64, vocab: u64, k: u64) -> u64;
     pub fn catena_b200_beam_select_f32_into(logits: *const f32, pitch: u64, scores: *const f32, batch: u64, beams: u64, vocab: u64, k: u64,
                                             out_scores: *mut f32, out_parents: *mut i32, out_tokens: *mut i32, workspace: *mut c_void,
-                                            workspace_bytes: u64) -> i32;
+                                            workspace_bytes: u64) -> catena_status_t;
     pub fn catena_b200_beam_select_bf16_into(logits: *const c_void, pitch: u64, scores: *const f32, batch: u64, beams: u64, vocab: u64,
                                              k: u64, out_scores: *mut f32, out_parents: *mut i32, out_tokens: *mut i32,
-                                             workspace: *mut c_void, workspace_bytes: u64) -> i32;
+                                             workspace: *mut c_void, workspace_bytes: u64) -> catena_status_t;
     pub fn catena_b200_beam_reorder_paged_bf16_into(cache: *const catena_paged_cache_t, parents: *const i32, beams: u64,
                                                     fresh_pages: *const i32, table_out: *mut i32, lengths_out: *mut i32,
-                                                    weights: *const f32, weights_out: *mut f32) -> i32;
+                                                    weights: *const f32, weights_out: *mut f32) -> catena_status_t;
     pub fn catena_b200_linear_bf16_into(x: *const c_void, w: *const c_void, residual: *const c_void, y: *mut c_void, m: u64,
                                         n: u64, k: u64) -> catena_status_t;
 
