@@ -9,7 +9,9 @@
 // behind k others cannot hold one of the k best, so about k segments are read again (from L2) and give the few candidates, which are
 // ranked by comparing them with each other.  Keeping k candidates per segment in launch 1 instead cost twice its time (45 against
 // 23 us for 32 x 8 rows of 128000 f32, 5.6 TB/s): almost all of them lose to another segment.
-// Candidates of different beams can lie closer together than f32 resolves, so the joined sums and the totals are f64.
+// Candidates of different beams can lie closer together than a total in f32 resolves, so the joined sums and the totals are f64; what
+// they can tell apart is limited by the segments' sums in f32, below 2^-19 of themselves.  Segments are counted from a row's start
+// whatever its alignment, so equal rows have equal sums and their ties are ties.
 #include <math.h>
 
 #include "catena_math.cuh"
@@ -124,6 +126,7 @@ __global__ void __launch_bounds__(kThreads) beam_stats_kernel(Rows<T> rows, uint
         uint64_t s2 = 0;
 #pragma unroll
         for (int u = 0; u < kPer; u += 2) {
+            if ((uint32_t)u / Rows<T>::N >= rows.pieces) break;
             float a, b;
             cmath::unpk2f(cmath::fma2(cmath::pk2f(x[u], x[u + 1]), l2, r2), a, b);
             s2 = cmath::add2(s2, cmath::pk2f(ex2(a), ex2(b)));
@@ -399,11 +402,16 @@ static catena_status_t check_sizes(uint64_t batch, uint64_t beams, uint64_t voca
     if (k > beams * vocab) return fail(CATENA_E_BAD_ARG, "beam_select: fewer continuations than places");
     return CATENA_OK;
 }
-// Segments of 1024 logits, halved (down to one 16-byte piece per lane) until a request has 512 of them: the limit is the better the more
-// segments there are than places, and few rows want many warps.
-static uint32_t pieces_for(uint64_t beams, uint64_t vocab, uint32_t per_piece) {
+// Segments of 1024 logits, halved (down to one 16-byte piece per lane) until a request has 512 of them, because few segments make a poor
+// limit (62 x 16 x 6574 f32: 16 us with segments of 512, 28 with 1024), or until the call has 48 warps for every SM, because a warp costs
+// about the same whatever its segment holds (52 x 4 x 29213 f32: 14 us with segments of 512, 31 with 128).
+static uint32_t pieces_for(uint64_t batch, uint64_t beams, uint64_t vocab, uint32_t per_piece) {
+    const uint64_t sms = tls().sm_count > 0 ? tls().sm_count : 148;
     uint32_t pieces = kPer / per_piece;
-    while (pieces > 1 && beams * ceil_div_u64(vocab, (uint64_t)pieces * 32 * per_piece) < 512) pieces /= 2;
+    for (; pieces > 1; pieces /= 2) {
+        const uint64_t segs = beams * ceil_div_u64(vocab, (uint64_t)pieces * 32 * per_piece);
+        if (segs >= 512 || batch * segs >= sms * 48) break;
+    }
     return pieces;
 }
 
@@ -420,7 +428,7 @@ static catena_status_t select_into(const T* logits, uint64_t pitch, const float*
     if (workspace_bytes < catena_b200_beam_select_workspace_bytes(batch, beams, vocab, k)) return fail(CATENA_E_BAD_ARG, "beam_select: workspace too small");
     uint32_t* err;
     CATENA_TRY(paged::begin(&err));
-    Rows<T> rows = {logits, pitch, (uint32_t)vocab, 0, pieces_for(beams, vocab, Piece<T>::kN), 0};
+    Rows<T> rows = {logits, pitch, (uint32_t)vocab, 0, pieces_for(batch, beams, vocab, Piece<T>::kN), 0};
     rows.segs = (uint32_t)ceil_div_u64(vocab, rows.pieces * 32 * Piece<T>::kN);
     rows.vec = paged::aligned16(logits) && pitch * sizeof(T) % 16 == 0;
     const uint64_t n = batch * beams * rows.segs;
@@ -439,7 +447,7 @@ extern "C" {
 uint64_t catena_b200_beam_select_workspace_bytes(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k) {
     if (!batch || beam::check_sizes(batch, beams, vocab, k) != CATENA_OK) return 0;
     // (maximum, sum) of every segment; f32's are never longer than bf16's
-    return batch * beams * ceil_div_u64(vocab, (uint64_t)beam::pieces_for(beams, vocab, 4) * 32 * 4) * sizeof(float2);
+    return batch * beams * ceil_div_u64(vocab, (uint64_t)beam::pieces_for(batch, beams, vocab, 4) * 32 * 4) * sizeof(float2);
 }
 catena_status_t catena_b200_beam_select_f32_into(const float* logits, uint64_t pitch, const float* scores, uint64_t batch, uint64_t beams,
                                                  uint64_t vocab, uint64_t k, float* out_scores, int32_t* out_parents, int32_t* out_tokens,

@@ -458,7 +458,8 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
 /* ---- beam search ----------------------------------------------------------------------------------------------
  * Selection: of the beams x vocabulary continuations of each request the k best by scores[request][beam] + log softmax(logits), in
  * descending order (ties: the lowest beam, then the greater logit, then the lowest token); logits [batch * beams] rows of `vocab`,
- * `pitch` elements apart, bf16 or f32.  Candidates of one beam are ordered by their logits, those of different beams by totals in f64.  A logit of -inf or NaN gives a total
+ * `pitch` elements apart, bf16 or f32.  Candidates of one beam are ordered by their logits, those of different beams by
+ * f64 totals over f32 sums of exponentials (off by less than 2^-19, the same for equal rows).  A logit of -inf or NaN gives a total
  * of -inf (chosen only when nothing else is left), +inf counts as the greatest finite f32; a NaN total counts as -inf.  Writes
  * out_scores / out_parents (beam within the request) / out_tokens [batch, k]; at most 64 beams and k <= 64.  The workspace is caller-owned, 256-byte
  * aligned. */

@@ -392,7 +392,7 @@ def select_reference(logits, scores, batch, beams, k):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("batch,beams,vocab,k", [(1, 1, 1, 1), (2, 4, 100, 8), (3, 1, 7, 7), (1, 4, 32000, 8), (2, 5, 50257, 10), (2, 64, 4100, 64), (1, 2, 4096, 64),
                                                  (5, 3, 33, 64), (1, 1, 300000, 33), (40, 2, 9000, 4), (3, 16, 200, 32), (2, 12, 64, 24), (1, 2, 300, 64)])
-@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("pad", [0, 3, 8])
 def test_select(dtype, batch, beams, vocab, k, pad):
     g = torch.Generator("cuda").manual_seed(beams * 1000 + vocab)
     logits = (torch.randn(batch * beams, vocab + pad, generator=g, device="cuda") * 3).to(dtype)
@@ -404,6 +404,28 @@ def test_select(dtype, batch, beams, vocab, k, pad):
     assert torch.equal(got[1].long(), parent) and torch.equal(got[2].long(), token)
     # rounding to f32, and a sum of n exponentials, each off by 2^-22 and its argument's rounding (|x - max| < 40): n-fold cancels in the mean
     assert ((got[0].double() - value).abs() <= 2.0 ** -24 * value.abs() + 2.0 ** -22 + 40 * 1.5 * 2.0 ** -23 + 64 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_of_rows_that_start_anywhere(dtype):
+    """Every start within a 16-byte piece, the best logits at the rows' ends; what lies around the rows is NaN."""
+    n = 16 // torch.finfo(dtype).bits * 8
+    for vocab in (1, 5, 127, 1024, 4093):
+        for off in range(n):
+            flat = torch.full((64 + 3 * (vocab + 5),), math.nan, device="cuda", dtype=dtype)
+            logits = flat[16 + off:].as_strided((3, vocab), (vocab + 5, 1))
+            logits.copy_(torch.randn(3, vocab, generator=torch.Generator("cuda").manual_seed(off), device="cuda"))
+            logits[:, 0], logits[:, -1] = 20.0, 30.0
+            k = min(4, 3 * vocab)
+            got = select(logits, torch.zeros(3, device="cuda"), 1, 3, k)
+            value, _, _ = select_reference(logits, torch.zeros(3, device="cuda"), 1, 3, k)
+            # The rows' best totals are alike to 1e-10, and a row's sum of exponentials is f32: each term off by 2^-22 (ex2.approx) and
+            # 2^-24 (its argument, near 0 where the term counts), 22 additions deep by 2^-24 each, below 2^-19 together.  So beams may
+            # change places where totals are closer than 2^-18, and what was chosen has to be as good as the best to that.
+            total = torch.log_softmax(logits.double(), -1)
+            chosen = total[got[1][0].long(), got[2][0].long()]
+            assert ((chosen - value[0]).abs() <= 2.0 ** -18).all() and len({*zip(got[1][0].tolist(), got[2][0].tolist())}) == k
+            assert ((got[0].double() - value).abs() <= 1e-5).all()
 
 
 def test_select_ties_go_to_the_lowest_beam_and_token():
