@@ -108,15 +108,21 @@ template <int TILE>
 struct Cursor {
     uint32_t b, h, tile, n;
     __device__ __forceinline__ uint32_t tiles() const { return (n + TILE - 1) / TILE; }
+    // whole warp, and only where the range goes on: sequences without rows are passed over 32 at a time
     __device__ __forceinline__ void next(const View& c) {
         if (++tile < tiles()) return;
         tile = 0;
         if (++h < c.hkv) return;
         h = 0;
-        do {
-            ++b;
-            n = b < c.n_seqs ? c.length(b) : 1u;
-        } while (n == 0);
+        for (++b; b < c.n_seqs; b += 32) {
+            const uint32_t at = b + (threadIdx.x & 31), mine = at < c.n_seqs ? c.length(at) : 0u;
+            const uint32_t some = __ballot_sync(0xFFFFFFFFu, mine != 0);
+            if (some == 0) continue;
+            n = __shfl_sync(0xFFFFFFFFu, mine, __ffs(some) - 1);
+            b += __ffs(some) - 1;
+            return;
+        }
+        n = 1;
     }
 };
 
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
             next_page = (uint32_t)c.table[(size_t)look.b * c.max_pages + j];
             next_within = look.h * c.page_size + (r - j * c.page_size);
         }
-        look.next(c);
+        if (to_look) look.next(c);
     };
     auto next_row = [&]() -> uint32_t {
         if (next_within == kNoRow) return kNoRow;
@@ -282,8 +288,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
         issue(c.k, row, kbase);
         look_up();
         const Cursor<TILE> now = at;
-        at.next(c);
-        if (at.tile == 0 && t + 1 < t1) load_q(at.b, at.h);        // the next segment's, while this one is finished
+        const bool last = t + 1 == t1;
+        if (!last) at.next(c);
+        if (!last && at.tile == 0) load_q(at.b, at.h);             // the next segment's, while this one is finished
         // thread: keys g, g + 8 of every 16 (rows of s), heads 2 t4, 2 t4 + 1 of each n-tile
         bool raise = false;
 #pragma unroll
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_decode_paged_k
         issue(c.v, row, vbase);
 
         const uint32_t unit_tiles = now.tiles(), b = now.b, h = now.h, tile = now.tile;
-        if (at.tile != 0 && t + 1 < t1) continue;
+        if (!last && at.tile != 0) continue;
         // ---- the segment [seg_first, tile] of unit (b, h) is done: join the warps
         fresh = true;
         const bool whole = seg_first == 0 && tile + 1 == unit_tiles;

@@ -101,6 +101,7 @@ SHAPES = [  # lengths, hq, hkv, d, page
     ([1], 1, 1, 128, 16), ([5, 0, 64, 65], 4, 2, 128, 16), ([63, 200, 17], 8, 1, 128, 8), ([300], 16, 16, 128, 16), ([1000, 1, 0, 333, 128], 12, 3, 128, 24),
     ([129, 127, 2], 16, 1, 64, 16), ([500, 0], 6, 2, 64, 1), ([31, 4096, 700], 10, 2, 64, 64), ([2500, 90, 90, 1300], 32, 2, 128, 48), ([40] * 70, 2, 1, 128, 7),
     ([20000], 8, 8, 128, 128), ([9999], 9, 1, 64, 1000), ([0, 0, 0], 4, 4, 128, 16), ([128] * 300, 16, 8, 64, 32),
+    ([0] * 150 + [1] + [0] * 40 + [70] + [0] * 33, 2, 2, 128, 16), (([0, 3] + [0] * 31) * 60, 4, 4, 64, 8),
 ]
 
 
