@@ -600,8 +600,12 @@ static Plan plan_for(const View& c, uint64_t d, uint64_t hq, bool weights) {
     }
     return p;
 }
-static catena_status_t check_heads(const View& c, uint64_t hq) {
+static catena_status_t check_heads(const View& c, uint64_t hq, bool weights) {
     if (hq == 0 || hq % c.hkv || hq / c.hkv > 16) return fail(CATENA_E_UNSUPPORTED, "attn_decode_paged: heads must be a multiple (<= 16) of kv heads");
+    // tiles of the whole call, and CTAs of the second launch, are counted in 32 bits
+    const uint64_t units = (uint64_t)c.n_seqs * c.hkv;
+    if (units > 0x7FFFFFFFull || units * (c.cap() / 64 + 1) > 0xFFFFFFFFull || (weights && units * ceil_div_u64(c.cap(), kWeightRows) > 0x7FFF0000ull))
+        return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: more rows or (sequence, kv head) pairs than the kernels index");
     return CATENA_OK;
 }
 
@@ -640,7 +644,7 @@ extern "C" {
 
 uint64_t catena_b200_attn_decode_paged_workspace_bytes(const catena_paged_cache_t* cache, uint64_t n_heads, int weights) {
     View c;
-    if (check_cache(cache, "attn_decode_paged: null cache", &c) != CATENA_OK || check_heads(c, n_heads) != CATENA_OK) return 0;
+    if (check_cache(cache, "attn_decode_paged: null cache", &c) != CATENA_OK || check_heads(c, n_heads, weights != 0) != CATENA_OK) return 0;
     return plan_for(c, cache->head_dim, n_heads, weights != 0).bytes;
 }
 
@@ -648,15 +652,12 @@ catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache
                                                         const float* weights_in, float* weights_out, void* workspace, uint64_t workspace_bytes) {
     View c;
     CATENA_TRY(check_cache(cache, "attn_decode_paged: null cache", &c));
-    CATENA_TRY(check_heads(c, n_heads));
+    CATENA_TRY(check_heads(c, n_heads, weights_out != nullptr));
     if (!c.n_seqs) return CATENA_OK;
     if (!q || !o || !workspace || (weights_in && !weights_out)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: null argument");
     if (!aligned16(q) || !aligned16(o) || !aligned4(weights_in) || !aligned4(weights_out) || ((uintptr_t)workspace & 255))
         return fail(CATENA_E_BAD_ARG, "attn_decode_paged: q and o must be 16-byte aligned, the workspace 256-byte");
     if (!(fabsf(scale) < 1e30f)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite (below 1e30)");
-    // tiles of the whole call are counted in 32 bits
-    if ((uint64_t)c.n_seqs * c.hkv > 0x7FFFFFFFull || (uint64_t)c.n_seqs * c.hkv * (c.cap() / 64 + 1) > 0xFFFFFFFFull || (weights_out && (uint64_t)c.n_seqs * c.hkv * ceil_div_u64(c.cap(), kWeightRows) > 0x7FFF0000ull))
-        return fail(CATENA_E_TOO_LARGE, "attn_decode_paged: more (sequence, kv head) pairs than the kernels index");
     CATENA_TRY(begin(&c.err));
     const Plan p = plan_for(c, cache->head_dim, n_heads, weights_out != nullptr);
     if (workspace_bytes < p.bytes) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: workspace too small");

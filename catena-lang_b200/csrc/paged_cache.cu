@@ -34,6 +34,7 @@ catena_status_t begin(uint32_t** err) {
 
 catena_status_t check_errors() {
     if (tls().device < 0 || !g_err[tls().device]) return CATENA_OK;
+    CATENA_TRY(ensure_device());
     uint32_t* word = g_err[tls().device];
     uint32_t h = 0;
     CATENA_CUDA(cudaMemcpyAsync(&h, word, sizeof(h), cudaMemcpyDeviceToHost, tls().stream));
@@ -567,7 +568,7 @@ catena_status_t catena_b200_rope_append_paged_bf16_into(const catena_paged_cache
 
 uint64_t catena_b200_kv_evict_paged_workspace_bytes(const catena_paged_cache_t* cache, uint64_t budget) {
     View c;
-    if (check_cache(cache, "kv_evict_paged: null cache", &c) != CATENA_OK || budget > 0x7FFFFFFFull) return 0;
+    if (check_cache(cache, "kv_evict_paged: null cache", &c) != CATENA_OK || budget > 0x7FFFFFFFull || (uint64_t)c.n_seqs * c.hkv > 65535) return 0;
     return (uint64_t)c.n_seqs * c.hkv * budget * sizeof(int32_t);
 }
 
@@ -586,9 +587,9 @@ catena_status_t catena_b200_kv_evict_paged_bf16_into(const catena_paged_cache_t*
     if (budget > max_pages_out * c.page_size) return fail(CATENA_E_BAD_ARG, "kv_evict_paged: table_out holds fewer rows than the budget");
     if (table_out == cache->table || lengths_out == cache->lengths || weights_out == weights)
         return fail(CATENA_E_BAD_ARG, "kv_evict_paged: rows move into other pages, lengths and weights into other buffers");
-    if (workspace_bytes < catena_b200_kv_evict_paged_workspace_bytes(cache, budget)) return fail(CATENA_E_BAD_ARG, "kv_evict_paged: workspace too small");
     const uint64_t units = (uint64_t)c.n_seqs * c.hkv;
     if (units > 65535) return fail(CATENA_E_TOO_LARGE, "kv_evict_paged: more than 65535 (sequence, kv head) pairs");
+    if (workspace_bytes < catena_b200_kv_evict_paged_workspace_bytes(cache, budget)) return fail(CATENA_E_BAD_ARG, "kv_evict_paged: workspace too small");
     CATENA_TRY(begin(&c.err));
     // A CTA per 2048 rows that a sequence may have, up to eight and as long as every CTA has an SM of its own.  (Clusters of small
     // CTAs are packed onto few SMs: 256 CTAs took 21 us where 128 with an SM each take 16.)  The shared memory that keeps a second CTA

@@ -126,6 +126,19 @@ def test_calls_without_work_are_answered_at_once():
     assert cb.lib().catena_b200_rope_angles_f32_into(10000.0, 0, 0, 128, None) == cb.OK
 
 
+def test_sizes_whose_products_pass_64_bits_are_refused():
+    L = cb.lib()
+    c = cache(n_seqs=1 << 20, n_kv_heads=1 << 15, max_pages=1 << 20, page_size=1 << 10, n_pages=1, head_dim=64)
+    for weights in (0, 1):
+        assert L.catena_b200_attn_decode_paged_workspace_bytes(C.byref(c), 1 << 19, weights) == 0
+    assert attend(c, heads=1 << 19, w_out=A) == cb.E_TOO_LARGE and attend(c, heads=1 << 19) == cb.E_TOO_LARGE
+    assert L.catena_b200_kv_evict_paged_workspace_bytes(C.byref(c), 1 << 30) == 0
+    assert evict(c, budget=1 << 20, pages=1 << 11) == cb.E_TOO_LARGE
+    assert append(c, pitch=1 << 62, heads=1 << 16) == cb.E_TOO_LARGE
+    wide = cache(n_seqs=64, n_kv_heads=1 << 14, max_pages=1 << 21, page_size=1 << 10, n_pages=1)
+    assert attend(wide, heads=1 << 14, w_out=A) == cb.E_TOO_LARGE
+
+
 def test_workspaces_cover_what_they_must():
     L = cb.lib()
     c = cache(n_seqs=3, max_pages=40)

@@ -325,8 +325,20 @@ def kept_rows(w, n, budget, recent):
     ([700, 699], 1, 128, 16, 90, 30, "specials"), ([5000], 1, 64, 16, 2500, 100, "two values")])
 @pytest.mark.parametrize("with_kept", [True, False])
 def test_evict(lengths, hkv, d, page, budget, recent, kind, with_kept):
+    check_evict(lengths, hkv, d, page, budget, recent, kind, with_kept, None)
+
+
+@pytest.mark.parametrize("lengths,hkv,page,max_pages,kind", [([700, 100, 2000] + [40] * 77, 1, 64, 800, "random"), ([5000], 1, 4096, 100, "two values"),
+                                                             ([5000, 9000], 2, 4096, 100, "random"), ([300] * 70, 2, 16, 20, "ties")])
+def test_evict_from_tables_of_any_width(lengths, hkv, page, max_pages, kind):
+    """The selection's launch goes by what the table could hold: more rows than a CTA keeps in shared memory, alone and in a cluster, and more
+    heads than there are SMs."""
+    check_evict(lengths, hkv, 64, page, 64, 10, kind, True, max_pages)
+
+
+def check_evict(lengths, hkv, d, page, budget, recent, kind, with_kept, max_pages):
     pages_out = -(-budget // page) + 1
-    c = Cache(9, lengths, hkv, d, page, spare=pages_out * len(lengths))
+    c = Cache(9, lengths, hkv, d, page, max_pages=max_pages, spare=pages_out * len(lengths))
     w = torch.rand(c.n, hkv, c.cap, generator=c.gen, device="cuda")
     if kind == "ties":
         w = (w * 5).floor()
