@@ -4,7 +4,7 @@
 // The exponential is the true one (ex2.approx in base 2), not math.exp-approx: that polynomial is not multiplicative, so it would
 // need the row's maximum before the first probability and with it a second pass over the scores.  Here one pass carries a running
 // maximum and sum.  q, k, v are bf16; scores, maxima, sums and outputs are f32 until the one rounding of o.  A probability enters
-// the second product as a bf16 pair (p rounded, and what the rounding left): with a single bf16 every p would be off by up to 2^-9
+// the second product as a bf16 pair (p rounded, and what the rounding left): with a single bf16 every p would be off by up to 2^-8
 // of itself, which for a row that looks at few keys is as much as the rounding of o.
 //
 // Bound: HBM.  A row costs 4 d bytes and 4 d flops per query head of the group, so even 16 heads (64 flops per 4 bytes) stay far
