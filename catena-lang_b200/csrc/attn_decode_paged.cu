@@ -544,9 +544,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(Vi
     }
     const uint32_t blocks = (c.cap() + kWeightRows - 1) / kWeightRows, at = blockIdx.x - ranges * slices;
     const uint32_t unit = at / blocks, j0 = at % blocks * kWeightRows, b = unit / c.hkv;
-    const uint32_t n = c.length(b);
+    const uint2 cut = part.split[unit];                    // of a unit without rows: whatever was there
+    const uint32_t n = c.length(b), j = j0 + tid * 4;
     if (j0 >= n) return;
-    const uint2 cut = part.split[unit];
+    // four heads' scores are on their way while (M, L) are joined
+    constexpr uint32_t kAhead = 4;
+    const float* sc = part.scores + (size_t)unit * group * part.pitch + j;       // the pitch is a multiple of 4
+    auto scores_of = [&](uint32_t i) { return *reinterpret_cast<const float4*>(sc + (size_t)i * part.pitch); };
+    float4 ahead[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (i < group && j < n) ahead[i] = scores_of(i);
     if (cut.x <= cut.y) {
         join_stats(part, cut.x, cut.y, 0, group, s_part, s_m, s_l);
     } else if (tid < group) {
@@ -555,19 +563,20 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_paged_join_kernel(Vi
         s_l[tid] = ml.y;
     }
     __syncthreads();
-    const uint32_t j = j0 + tid * 4;
     if (j >= n) return;
     float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float* sc = part.scores + (size_t)unit * group * part.pitch + j;       // the pitch is a multiple of 4
-#pragma unroll 4
-    for (uint32_t i = 0; i < group; ++i) {
-        const float4 s = *reinterpret_cast<const float4*>(sc + (size_t)i * part.pitch);
+    auto add = [&](uint32_t i, const float4& s) {
         const float m = s_m[i] == -INFINITY ? 0.0f : s_m[i], r = s_l[i] == 0.0f ? 0.0f : __frcp_rn(s_l[i]);
         w.x = __fmaf_rn(ex2(__fsub_rn(s.x, m)), r, w.x);
         w.y = __fmaf_rn(ex2(__fsub_rn(s.y, m)), r, w.y);
         w.z = __fmaf_rn(ex2(__fsub_rn(s.z, m)), r, w.z);
         w.w = __fmaf_rn(ex2(__fsub_rn(s.w, m)), r, w.w);
-    }
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (i < group) add(i, ahead[i]);
+#pragma unroll 4
+    for (uint32_t i = kAhead; i < group; ++i) add(i, scores_of(i));
     const float ws[4] = {w.x, w.y, w.z, w.w};
     const size_t to = (size_t)unit * c.cap() + j;
 #pragma unroll
