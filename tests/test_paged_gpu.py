@@ -576,6 +576,96 @@ def test_a_captured_step_replays_on_new_lengths_and_two_streams_do_not_meet():
     cb.check(L.catena_b200_check_device_errors())
 
 
+def test_what_a_non_blocking_call_met_is_reported_by_the_check():
+    L = cb.lib()
+    c = Cache(30, [20, 40], 1, 128, 16)
+    q = torch.randn(2, 2, 128, generator=c.gen, device="cuda").bfloat16()
+    c.table[1, 1] = 1 << 20
+    L.catena_b200_set_blocking(0)
+    assert attend(c, q, 0.1)[0] == cb.OK
+    assert L.catena_b200_check_device_errors() == cb.E_ASSERT and L.catena_b200_check_device_errors() == cb.OK
+
+
+def test_sequences_that_share_pages():
+    """Two sequences that name the same pages, and one that names a page twice, are read like any others; evicting them moves copies."""
+    c = Cache(31, [48, 40, 37], 2, 64, 16, spare=6)
+    c.table[1] = c.table[0]
+    c.table[2, 2] = c.table[2, 0]
+    q = torch.randn(3, 4, 64, generator=c.gen, device="cuda").bfloat16()
+    status, got = attend(c, q, 0.125)
+    cb.check(status)
+    for b, n in enumerate((48, 40, 37)):
+        o, off, _, _ = attention_reference(c, q, 0.125, b, n)
+        assert ((got[b].double() - o).abs() <= 2.0 ** -8 * o.abs() + off * (1 + 2.0 ** -8)).all()
+    w = torch.rand(3, 2, c.cap, generator=c.gen, device="cuda")
+    t_out = c.spare.cuda().view(3, 2).contiguous()
+    l_out, w_out = torch.zeros_like(c.lengths), torch.zeros(3, 2, 32, device="cuda")
+    kept = torch.zeros(3, 2, 25, dtype=torch.int32, device="cuda")
+    ws = torch.empty(3 * 2 * 25 * 4, dtype=torch.uint8, device="cuda")
+    s = c.struct()
+    cb.check(cb.lib().catena_b200_kv_evict_paged_bf16_into(C.byref(s), ptr(w), 25, 9, ptr(t_out), 2, ptr(l_out), ptr(w_out), ptr(kept), ptr(ws), ws.numel()))
+    for b, n in enumerate((48, 40, 37)):
+        old, new = c.rows(c.k, b, n), c.rows(c.k, b, 25, t_out)
+        for h in range(2):
+            rows = kept_rows(w[b, h].tolist(), n, 25, 9)
+            assert kept[b, h].tolist() == rows and torch.equal(new[h], old[h][rows])
+
+
+def test_captured_eviction_and_search_replay_on_new_inputs():
+    """Launches in clusters, and copies that begin beside the selection: a replayed graph gives what the calls give."""
+    L = cb.lib()
+    c = Cache(32, [3000] * 4, 2, 128, 16, spare=4 * 20 + 4)          # pages for every length below
+    spare = c.spare.cuda()
+    t_out, fresh = spare[:80].view(4, 20).contiguous(), spare[80:].contiguous()
+    w = torch.rand(4, 2, c.cap, generator=c.gen, device="cuda")
+    l_out, w_out = torch.zeros_like(c.lengths), torch.zeros(4, 2, 320, device="cuda")
+    kept = torch.zeros(4, 2, 300, dtype=torch.int32, device="cuda")
+    logits, scores = torch.zeros(4, 20000, device="cuda"), torch.zeros(4, device="cuda")
+    picked = torch.zeros(2, 2, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    t2, l2 = torch.zeros_like(c.table), torch.zeros_like(c.lengths)
+    s = c.struct()
+    ws = torch.empty(L.catena_b200_kv_evict_paged_workspace_bytes(C.byref(s), 300), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(L.catena_b200_beam_select_workspace_bytes(2, 2, 20000, 2), dtype=torch.uint8, device="cuda")
+    cb.check(L.catena_b200_rope_angles_f32_into(10000.0, 0, 1, 128, ptr(torch.zeros(64, 2, device="cuda"))))     # the thread's first call
+
+    def calls():
+        cb.check(L.catena_b200_kv_evict_paged_bf16_into(C.byref(s), ptr(w), 300, 100, ptr(t_out), 20, ptr(l_out), ptr(w_out), ptr(kept), ptr(ws), ws.numel()))
+        cb.check(L.catena_b200_beam_select_f32_into(ptr(logits), 20000, ptr(scores), 2, 2, 20000, 2, *map(ptr, picked), ptr(ws2), ws2.numel()))
+        cb.check(L.catena_b200_beam_reorder_paged_bf16_into(C.byref(s), ptr(picked[1]), 2, ptr(fresh), ptr(t2), ptr(l2), None, None))
+    stream = torch.cuda.Stream()
+    cb.check(L.catena_b200_set_stream(stream.cuda_stream))
+    L.catena_b200_set_blocking(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        graph.capture_begin()
+        calls()
+        graph.capture_end()
+    results = {"graph": [], "eager": []}
+    for i in range(4):
+        g = torch.Generator("cuda").manual_seed(i)
+        w.copy_(torch.rand(w.shape, generator=g, device="cuda"))
+        logits.copy_(torch.randn(logits.shape, generator=g, device="cuda"))
+        c.lengths.copy_(torch.tensor([[3000, 100, 2500, 64], [2999, 299, 300, 301], [310, 0, 1, 3000], [5, 6, 700, 800]][i], dtype=torch.int32))
+        k0, v0 = c.k.clone(), c.v.clone()
+        for mode in results:
+            c.k.copy_(k0), c.v.copy_(v0)
+            for t in (l_out, w_out, kept, t2, l2, *picked):
+                t.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay() if mode == "graph" else calls()
+            torch.cuda.synchronize()
+            results[mode].append([x.clone() for x in (c.k.view(torch.int16), c.v.view(torch.int16), l_out, w_out, kept, t2, l2, *picked)])
+        n = c.lengths.tolist()
+        for b in range(4):
+            rows = kept_rows(w[b, 1].tolist(), n[b], 300, 100)
+            assert int(l_out[b]) == len(rows) and kept[b, 1, : len(rows)].tolist() == rows
+    for a, b in zip(results["graph"], results["eager"]):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    cb.check(L.catena_b200_check_device_errors())
+
+
 def test_two_host_threads_on_streams_of_their_own():
     """Library state belongs to the thread: calls that overlap on the device, each with its own workspace, give the bits of calls alone."""
     import threading
