@@ -664,6 +664,7 @@ catena_status_t catena_b200_attn_decode_paged_bf16_into(const catena_paged_cache
     CATENA_TRY(check_heads(c, n_heads, weights_out != nullptr));
     if (!c.n_seqs) return CATENA_OK;
     if (!q || !o || !workspace || (weights_in && !weights_out)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: null argument");
+    if (q == o) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: o must be another buffer than q");
     if (!aligned16(q) || !aligned16(o) || !aligned4(weights_in) || !aligned4(weights_out) || ((uintptr_t)workspace & 255))
         return fail(CATENA_E_BAD_ARG, "attn_decode_paged: q and o must be 16-byte aligned, the workspace 256-byte");
     if (!(fabsf(scale) < 1e30f)) return fail(CATENA_E_BAD_ARG, "attn_decode_paged: scale must be finite (below 1e30)");

@@ -434,7 +434,7 @@ catena_status_t catena_b200_rope_angles_f32_into(float base, uint64_t pos0, uint
 catena_status_t catena_b200_rope_append_paged_bf16_into(const catena_paged_cache_t* cache, const void* qkv, uint64_t qkv_pitch,
                                                         const int32_t* token_start, uint64_t tokens, const int32_t* positions,
                                                         const void* angles, uint64_t n_angles, uint64_t n_heads, void* q_out);
-/* Attention of one token per sequence over all its rows: q, o [n_seqs, n_heads, head_dim]; n_heads a multiple of n_kv_heads, at
+/* Attention of one token per sequence over all its rows: q, o [n_seqs, n_heads, head_dim], two buffers; n_heads a multiple of n_kv_heads, at
  * most 16 times.  o = softmax(scale q k^T) v with the true exponential (not math.exp-approx); probabilities, sums and the running
  * maximum are f32.  A sequence without rows, or whose scores are all -inf, gives zeros.  With weights_out [n_seqs, n_kv_heads,
  * max_pages * page_size] f32: weights_out = weights_in + the attention each row gets, summed over the query heads of its kv head

@@ -15,7 +15,7 @@ def cache(**kw):
     return cb.PagedCacheStruct(*[f[n] for n, _ in cb.PagedCacheStruct._fields_])
 
 
-def attend(c=None, q=A, o=A, heads=4, scale=0.1, w_in=None, w_out=None, ws=A, ws_bytes=1 << 40):
+def attend(c=None, q=A, o=2 * A, heads=4, scale=0.1, w_in=None, w_out=None, ws=A, ws_bytes=1 << 40):
     c = c or cache()
     return cb.lib().catena_b200_attn_decode_paged_bf16_into(C.byref(c), q, o, heads, scale, w_in, w_out, ws, ws_bytes)
 
@@ -66,7 +66,7 @@ def test_null_cache():
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(q=None), cb.E_BAD_ARG), (dict(o=None), cb.E_BAD_ARG), (dict(ws=None), cb.E_BAD_ARG), (dict(q=A + 8), cb.E_BAD_ARG), (dict(o=A + 2), cb.E_BAD_ARG),
+    (dict(q=None), cb.E_BAD_ARG), (dict(o=None), cb.E_BAD_ARG), (dict(o=A), cb.E_BAD_ARG), (dict(ws=None), cb.E_BAD_ARG), (dict(q=A + 8), cb.E_BAD_ARG), (dict(o=A + 2), cb.E_BAD_ARG),
     (dict(ws=A + 16), cb.E_BAD_ARG), (dict(heads=3), cb.E_UNSUPPORTED), (dict(heads=0), cb.E_UNSUPPORTED), (dict(heads=34), cb.E_UNSUPPORTED),
     (dict(scale=float("nan")), cb.E_BAD_ARG), (dict(scale=float("inf")), cb.E_BAD_ARG), (dict(scale=-3e38), cb.E_BAD_ARG), (dict(w_in=A), cb.E_BAD_ARG), (dict(w_out=A + 1), cb.E_BAD_ARG)])
 def test_attention_refusals(change, status):

@@ -586,6 +586,41 @@ def test_what_a_non_blocking_call_met_is_reported_by_the_check():
     assert L.catena_b200_check_device_errors() == cb.E_ASSERT and L.catena_b200_check_device_errors() == cb.OK
 
 
+def test_a_threads_first_call_is_refused_inside_a_capture():
+    """It would allocate the thread's error word; the capture survives the refusal, and after a call outside it is accepted."""
+    import threading
+    L = cb.lib()
+    c = Cache(33, [20], 1, 128, 16)
+    q = torch.randn(1, 2, 128, generator=c.gen, device="cuda").bfloat16()
+    o, s = torch.zeros_like(q), c.struct()
+    ws = torch.empty(L.catena_b200_attn_decode_paged_workspace_bytes(C.byref(s), 2, 0), dtype=torch.uint8, device="cuda")
+    seen = []
+
+    def work():
+        def call():
+            return L.catena_b200_attn_decode_paged_bf16_into(C.byref(s), ptr(q), ptr(o), 2, 0.1, None, None, ptr(ws), ws.numel())
+        seen.append(L.catena_b200_init(0))
+        L.catena_b200_set_blocking(0)
+        stream = torch.cuda.Stream()
+        seen.append(L.catena_b200_set_stream(stream.cuda_stream))
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(stream):
+                graph.capture_begin()
+                seen.append(call())
+                graph.capture_end()
+            seen.append(call())
+            stream.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append(L.catena_b200_check_device_errors())
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert seen == [cb.OK, cb.OK, cb.E_UNSUPPORTED, cb.OK, cb.OK, cb.OK, cb.OK]
+
+
 def test_sequences_that_share_pages():
     """Two sequences that name the same pages, and one that names a page twice, are read like any others; evicting them moves copies."""
     c = Cache(31, [48, 40, 37], 2, 64, 16, spare=6)
